@@ -4,29 +4,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-typedef uint32_t gz_sgpr4 __attribute__((ext_vector_type(4)));
-
-// four wave-uniform dwords to a wave-uniform, 16-byte aligned address with ONE scalar instruction (s_store_dwordx4)
-// instead of 4 v_mov + an exec-masked vector store. The values must be scalar (SALU results).
-__device__ static inline void gz_scalar_store4 (uint32_t *dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
-{
-    gz_sgpr4 v = { a, b, c, d };
-    asm volatile ("s_store_dwordx4 %0, %1, 0x0" : : "s"(v), "s"(dst) : "memory");
-}
-
-// one wave-uniform dword to a wave-uniform address (s_store_dword)
-__device__ static inline void gz_scalar_store1 (uint32_t *dst, uint32_t a)
-{
-    asm volatile ("s_store_dword %0, %1, 0x0" : : "s"(a), "s"(dst) : "memory");
-}
-
-// the same with an immediate byte offset (one base pointer serves several stores)
-template <int OFF> __device__ static inline void gz_scalar_store4_at (uint32_t *dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
-{
-    gz_sgpr4 v = { a, b, c, d };
-    asm volatile ("s_store_dwordx4 %0, %1, %2" : : "s"(v), "s"(dst), "n"(OFF) : "memory");
-}
-
 // wait for every outstanding scalar load (they return out of order, so "all" is the only wait there is) without
 // waiting for vector memory operations. A builtin, not inline asm: the compiler's own wait-count bookkeeping sees it.
 __device__ static inline void gz_wait_scalar_loads (void) { __builtin_amdgcn_s_waitcnt (0xC07F); }   // vmcnt 63, expcnt 7, lgkmcnt 0
@@ -37,12 +14,6 @@ __device__ static inline void gz_wait_vector_mem (void) { __builtin_amdgcn_s_wai
 
 // keep the instruction scheduler from moving anything across this point (it likes to sink loads towards their use)
 __device__ static inline void gz_sched_fence (void) { __builtin_amdgcn_sched_barrier (0); }
-
-// scalar stores sit in the scalar data cache: write it back before anybody else (a later kernel) reads the data
-__device__ static inline void gz_scalar_store_flush (void)
-{
-    asm volatile ("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb\n\ts_waitcnt lgkmcnt(0)" : : : "memory");
-}
 
 // number of set bits of a wave mask below my lane (v_mbcnt_lo + v_mbcnt_hi)
 __device__ static inline uint32_t gz_mbcnt (uint64_t m)
@@ -119,6 +90,12 @@ __device__ static inline uint4 gz_ldg_u32x4 (const void *p)
 }
 __device__ static inline void gz_stg_u8 (uint8_t *p, uint32_t v) { *(__attribute__((address_space(1))) uint8_t *)(uintptr_t)p = (uint8_t)v; }
 __device__ static inline void gz_stg_u32 (uint32_t *p, uint32_t v) { *(__attribute__((address_space(1))) uint32_t *)(uintptr_t)p = v; }
+__device__ static inline void gz_stg_u32x2 (uint32_t *p, uint32_t a, uint32_t b)     // 8 bytes, 8-byte aligned, through a GLOBAL pointer
+{
+    typedef uint32_t gz_v2 __attribute__((ext_vector_type(2)));
+    const gz_v2 v = { a, b };
+    *(__attribute__((address_space(1))) gz_v2 *)(uintptr_t)p = v;
+}
 __device__ static inline void gz_stg_rec (void *p, uint32_t a, uint32_t b, uint32_t c)     // 12 bytes, 4-byte aligned, through a GLOBAL pointer (global_store_dwordx3)
 {
     typedef uint32_t gz_v3 __attribute__((ext_vector_type(3)));
@@ -153,7 +130,7 @@ __device__ static inline double gz_fma_rtz (double a, double b, double c) { retu
 #endif
 // Whole blocks of GZ_CHAIN_BLOCK symbols of one leaf's chain (tools/gen_chain_asm.py explains the loop). (rlo, rhi) = the state,
 // a double (range * 2^-7), wave-uniform in and out; recs = the 12-byte records of the first block; ck = where the first block's first
-// checkpoint goes (8 bytes per 64 symbols, scalar stores).
+// checkpoint goes (8 bytes per 64 symbols; the loop's stores are complete when it ends). Every lane of the wave must be active.
 __device__ static inline void gz_chain_blocks (uint32_t &rlo, uint32_t &rhi, const uint8_t *recs, uint32_t nblk, uint32_t *ck)
 {
     const uint64_t b = (uint64_t)(uintptr_t)recs, c = (uint64_t)(uintptr_t)ck;
@@ -163,10 +140,4 @@ __device__ static inline void gz_chain_blocks (uint32_t &rlo, uint32_t &rhi, con
     asm volatile (GZ_CHAIN_F64_ASM : [rlo] "+v"(rlo), [rhi] "+v"(rhi)
                                    : [blo] "s"(b_lo), [bhi] "s"(b_hi), [nblk] "s"(nb), [clo] "s"(c_lo), [chi] "s"(c_hi) : GZ_CHAIN_F64_CLOBBERS);
     rlo = (uint32_t)__builtin_amdgcn_readfirstlane ((int)rlo); rhi = (uint32_t)__builtin_amdgcn_readfirstlane ((int)rhi);   // (the state ends in lane 0)
-}
-// one 8-byte checkpoint through the scalar unit
-__device__ static inline void gz_scalar_store2 (uint32_t *dst, uint32_t a, uint32_t b)
-{
-    const uint32_t sa = (uint32_t)__builtin_amdgcn_readfirstlane ((int)a), sb = (uint32_t)__builtin_amdgcn_readfirstlane ((int)b);   // (wave-uniform values that live in vector registers)
-    asm volatile ("s_store_dwordx2 %0, %1, 0x0" : : "s"((uint64_t)sa | (uint64_t)sb << 32), "s"(dst) : "memory");
 }

@@ -1397,7 +1397,7 @@ __device__ static inline bool d_wait_progress (const uint32_t *progress, uint32_
 __device__ static inline void d_chain_slow (uint32_t &rlo, uint32_t &rhi, int lane, uint32_t i0, uint32_t i1, const uint8_t *triples, uint32_t *ck)
 {
     for (uint32_t g = i0; g < i1; g += 64) {
-        gz_scalar_store2 (ck + 2 * (g >> 6), rlo, rhi);
+        if (!lane) gz_stg_u32x2 (ck + 2 * (g >> 6), rlo, rhi);
         const GzRec mine = ((const GzRec *)triples)[g + lane];  // (beyond i1: inside the padded area, not looked at)
         const uint32_t fq = g + lane < i1 ? d_record_freq (mine.f) : 1u;
         const int m = i1 - g < 64 ? (int)(i1 - g) : 64;
@@ -1407,14 +1407,15 @@ __device__ static inline void d_chain_slow (uint32_t &rlo, uint32_t &rhi, int la
 
 // positions [p0, p1) of one leaf (p0 a multiple of 64; p1 - p0 one of GZ_CHAIN_BLOCK unless p1 is the leaf's end)
 // What leaves the chain is the state BEFORE every 64th symbol (8 bytes at ck + 2 * (i / 64)) and the state after the last symbol
-// of the call (the next call's first checkpoint, or the leaf's closing one): one scalar store per 64 symbols.
+// of the call (the next call's first checkpoint, or the leaf's closing one): lane 0 stores it here, the loop stores a block's
+// checkpoints with one instruction.
 __device__ static __forceinline__ void d_chain_chunk (uint32_t &rlo, uint32_t &rhi, int lane, uint32_t p0, uint32_t p1, const uint8_t *triples, uint32_t *ck)
 {
     const uint32_t whole = p0 + (p1 - p0) / GZ_CHAIN_BLOCK * GZ_CHAIN_BLOCK;
     uint32_t i = p0;
     if (whole > p0) { gz_chain_blocks (rlo, rhi, triples + (size_t)p0 * GZ_CHAIN_REC, (whole - p0) / GZ_CHAIN_BLOCK, ck + 2 * (p0 >> 6)); i = whole; }
     if (i < p1) d_chain_slow (rlo, rhi, lane, i, p1, triples, ck);     // the end of the leaf
-    gz_scalar_store2 (ck + 2 * ((p1 + 63) >> 6), rlo, rhi);
+    if (!lane) gz_stg_u32x2 (ck + 2 * ((p1 + 63) >> 6), rlo, rhi);
 }
 
 // progress == NULL: everything is there already, one piece (bounds is ignored). bounds [0 .. n_chunks]: where the position chunks start (the
@@ -1445,15 +1446,13 @@ __device__ static __forceinline__ void d_arith_chain (GzdLeaf *leaves, const uin
             if (k && !d_wait_progress (progress, k + 1)) { if (!lane) { L.overflow = 2; *fail = 1; } break; }
             d_chain_chunk (rlo, rhi, lane, p0, pe < n ? pe : n, triples, ck);
             if (done) {                                        // this leaf's checkpoints of chunk k are final: tell the low kernels
-                gz_scalar_store_flush ();
-                __threadfence ();
+                __threadfence ();                              // (the loop has waited for its own stores, the fence waits for the compiler's)
                 if (!lane) {
                     atomicAdd (&done[k], 1u);
                     if (n <= pe) for (uint32_t k2 = k + 1; k2 < n_chunks; k2++) atomicAdd (&done[k2], 1u);   // (a short leaf has no later chunks)
                 }
             }
         }
-    gz_scalar_store_flush ();
 }
 
 __global__ void __launch_bounds__(64 * GZ_CHAIN_WAVES) k_arith_chain (GzdLeaf *leaves, const uint32_t *list, uint32_t n_list, const uint32_t *progress,

@@ -2,14 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
-static inline void gz_scalar_store4 (uint32_t *dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
-{
-    if (emu.cur % 64 == 0) { dst[0] = a; dst[1] = b; dst[2] = c; dst[3] = d; }
-}
-static inline void gz_scalar_store1 (uint32_t *dst, uint32_t a) { if (emu.cur % 64 == 0) dst[0] = a; }
-static inline void gz_scalar_store_flush (void) {}
 static inline uint32_t gz_mbcnt (uint64_t m) { return (uint32_t)__builtin_popcountll (m & ((1ull << (emu.cur % 64)) - 1)); }
-template <int OFF> static inline void gz_scalar_store4_at (uint32_t *dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) { gz_scalar_store4 (dst + OFF / 4, a, b, c, d); }
 static inline void gz_wait_scalar_loads (void) {}
 static inline void gz_sched_fence (void) {}
 static inline void gz_scalar_cache_inv (void) {}
@@ -30,6 +23,7 @@ static inline uint2 gz_ldg_u32x2 (const void *p) { return *(const uint2 *)p; }
 static inline uint4 gz_ldg_u32x4 (const void *p) { return *(const uint4 *)p; }
 static inline void gz_stg_u8 (uint8_t *p, uint32_t v) { *p = (uint8_t)v; }
 static inline void gz_stg_u32 (uint32_t *p, uint32_t v) { *p = v; }
+static inline void gz_stg_u32x2 (uint32_t *p, uint32_t a, uint32_t b) { p[0] = a; p[1] = b; }
 static inline void gz_stg_u16 (uint8_t *p, uint32_t v) { p[0] = (uint8_t)v; p[1] = (uint8_t)(v >> 8); }
 static inline void gz_stg_rec (void *p, uint32_t a, uint32_t b, uint32_t c) { uint32_t *q = (uint32_t *)p; q[0] = a; q[1] = b; q[2] = c; }
 static inline uint32_t gz_wave_shr1 (uint32_t x, uint32_t fill)
@@ -58,7 +52,6 @@ static inline double gz_fma_rtz (double a, double b, double c)
     volatile double va = a, vb = b, vc = c; const double r = fma (va, vb, vc);
     fesetround (was); return r;
 }
-static inline void gz_scalar_store2 (uint32_t *dst, uint32_t a, uint32_t b) { if (emu.cur % 64 == 0) { dst[0] = a; dst[1] = b; } }
 #include "gz_chain_asm.h"                                       // (GZ_CHAIN_BLOCK; the loop itself is not for this compiler)
 // the same contract as the product's loop, one symbol at a time, in the loop's own arithmetic: records { inv.lo | cum, inv.hi, F.hi },
 // T = fma (R, inv, 1.0) truncated (inv as it stands in the record, cum in its low bits), R' = fma (T, F, -F) with F = freq * 2^45, then the exponent bits
@@ -67,7 +60,7 @@ static inline void gz_chain_blocks (uint32_t &rlo, uint32_t &rhi, const uint8_t 
     for (uint32_t b = 0; b < nblk; b++) {
         const uint32_t *rec = (const uint32_t *)(recs + (size_t)b * GZ_CHAIN_BLOCK * GZ_CHAIN_REC);
         for (int j = 0; j < GZ_CHAIN_BLOCK; j++) {
-            if (!(j & 63)) gz_scalar_store2 (ck + 2 * (b * (GZ_CHAIN_BLOCK / 64) + j / 64), rlo, rhi);
+            if (!(j & 63) && emu.cur % 64 == 0) gz_stg_u32x2 (ck + 2 * (b * (GZ_CHAIN_BLOCK / 64) + j / 64), rlo, rhi);
             double inv, R, F; memcpy (&inv, rec + 3 * j, 8);
             uint64_t rb = (uint64_t)rlo | (uint64_t)rhi << 32; memcpy (&R, &rb, 8);
             const uint64_t fb = (uint64_t)rec[3 * j + 2] << 32; memcpy (&F, &fb, 8);

@@ -32,7 +32,7 @@ Round 6 - what the loop paid for beyond its three instructions, measured (tools/
     tests/test_abi.py checks every 8-byte instruction's address in the assembled loop.
   * an instruction that has nothing to do with the chain costs 4 clocks wherever it stands (a load 13) - except in the two wait states
     in front of a hop's DPP read, which have to be there anyway: the next block's loads (two a hop), the shifts that make its operands,
-    the scalar stores of the checkpoints all go THERE instead of s_nop; a hop costs 12 clocks in all (1.0 a symbol at 12 a lane).
+    the shift of the checkpoints' lane mask all go THERE instead of s_nop; a hop costs 12 clocks in all (1.0 a symbol at 12 a lane).
   * the next block's operand shifts happen late in the current block (its loads were issued in the first hops and are waited for in
     hop 40: long there); nothing is left at a block's head.
   * A HOP INSIDE A ROW OF 16 LANES IS THE SECOND FMA ITSELF: gfx950 has one double-precision instruction with a DPP operand,
@@ -49,6 +49,12 @@ Round 6 - what the loop paid for beyond its three instructions, measured (tools/
     (2 PER + 2 `v_mov_b64`, 4 bytes each, an even number: 0.13 clocks a symbol at 16 a lane). 26 KB at 16 symbols a lane (1024-symbol blocks,
     a checkpoint always at a lane's first symbol): 13.00 clocks a symbol alone, the chain's launch 35.3 -> 34.35 ms in the step (12 / 24 a lane in
     one copy: 13.23 / 12.82 alone, 34.7 / 35.1 in the step). profiles/r06_ubench_chain_single.txt, r06_ab_chain_single.txt.
+
+The checkpoints - the state before every 64th symbol - sit in a different lane each (symbol 64 c is the turn of lane 64 c / PER), so they
+are KEPT in a register pair of their own, two v_cndmask_b32 under a one-lane mask each, and leave the block together: one
+global_store_dwordx2 under the mask of those lanes, lane 64 c / PER to the block's checkpoint c. The store is waited for where the next
+block's loads are (and behind the loop), thousands of clocks later. Only vector stores write memory here: data written through
+the scalar cache is not coherent with the other kernels that read the checkpoints while the chain is still running.
 
 Everything between the labels is written here, loop control included: the compiler schedules nothing in it. The rest of a leaf that
 does not fill a block is the caller's.
@@ -93,15 +99,28 @@ def regset(base):
 SETS = [regset(FIRST), regset(FIRST + 4 * PER + 4)]
 LAST_V = SETS[1]['last']
 assert LAST_V <= 255, 'out of vector registers'
-CLOB_V = FIXED_V + list(range(FIRST, LAST_V + 1))
-CLOB_S = [36, 37, 40, 41, 42, 43, 44, 45, 46, 47]
-NEXT, CK, TMP = "s[40:41]", "s[44:45]", "s[46:47]"      # NEXT = the records of the next block (of this one, when there is none: loaded, not used)
+CKV, CKLO, CKHI = f"v[{LAST_V + 1}:{LAST_V + 2}]", f"v{LAST_V + 1}", f"v{LAST_V + 2}"     # a lane's checkpoint of this block
+CKOFF = f"v{_b + 1}"                                                                       # ... and where it goes, from CK on
+assert (LAST_V + 1) % 2 == 0 and LAST_V + 2 <= 255
+CLOB_V = FIXED_V + list(range(FIRST, LAST_V + 3))
+CLOB_S = [36, 37, 40, 41, 42, 43, 44, 45, 46, 47, 48, 49]
+NEXT, CK = "s[40:41]", "s[44:45]"                       # NEXT = the records of the next block (of this one, when there is none: loaded, not used)
+LANE, CKLANES = "s[46:47]", "s[48:49]"                  # the lane of the checkpoint that comes next (one bit); all lanes that hold one
+CKPTS = [c for c in range(BLOCK // 64) if X_CKPT and (64 * c) % X_CKPT == 0]
+
+
+def ck_lane(c):
+    """whose turn symbol 64 c of a block is"""
+    return 64 * c // PER
+
+
 DPP = "wave_ror:1 row_mask:0xf bank_mask:0xf"
 NOP2 = ["s_nop 0", "s_nop 0"]                           # two wait states in eight bytes
 
 _INLINE_F = {"0.5", "-0.5", "1.0", "-1.0", "2.0", "-2.0", "4.0", "-4.0"}
-_FOUR = ("s_nop", "s_waitcnt", "s_cbranch", "s_branch", "s_cmp", "s_mov_b32", "s_add_u32", "s_addc_u32", "s_sub_u32", "s_cselect_b32", "v_mov_b32", "v_mul_u32_u24", "v_xor_b32", "v_mov_b64")
-_EIGHT = ("v_fma_f64", "v_and_or_b32", "v_lshlrev_b64", "global_load", "global_store", "s_store", "v_readlane_b32", "v_mbcnt")
+_FOUR = ("s_nop", "s_waitcnt", "s_cbranch", "s_branch", "s_cmp", "s_mov_b32", "s_add_u32", "s_addc_u32", "s_sub_u32", "s_cselect_b32", "s_mov_b64", "s_lshl_b64",
+         "v_mov_b32", "v_mul_u32_u24", "v_xor_b32", "v_mov_b64", "v_add_u32", "v_lshrrev_b32", "v_lshlrev_b32")
+_EIGHT = ("v_fma_f64", "v_and_or_b32", "v_lshlrev_b64", "global_load", "global_store", "v_mbcnt")
 
 
 def size(ins):
@@ -170,7 +189,7 @@ def nfp_make(s):
 
 
 def hop_fillers(cur, nxt):
-    """what stands in the wait states of each of a block's 64 hops: the next block's loads, its operand shifts, the checkpoints' stores"""
+    """what stands in the wait states of each of a block's 64 hops: the next block's loads, its operand shifts, the checkpoints' lane mask"""
     H = [[] for _ in range(64)]
     if X_FILL:
         ld = [f"global_load_dwordx3 {nxt['rec'][k]}, {OFF}, {NEXT} offset:{REC * k}" for k in range(PER)]
@@ -186,10 +205,11 @@ def hop_fillers(cur, nxt):
         H[hf].append(fp_mov(nxt))
         if X_FUSE:
             H[hf + 1].append(nfp_make(nxt))
-    if X_CKPT:
-        for c in range(BLOCK // 64):
-            if (64 * c) % X_CKPT == 0:
-                H[(64 * c) // PER].append(f"s_store_dwordx2 {TMP}, {CK}, 0x{8 * c:x}")        # what the two v_readlane in front of symbol 64 c have read
+    for i, c in enumerate(CKPTS):                            # on to the lane of the next checkpoint; behind the last one back to the first (lane 0)
+        if i + 1 < len(CKPTS):
+            H[ck_lane(c)].insert(0, f"s_lshl_b64 {LANE}, {LANE}, {ck_lane(CKPTS[i + 1]) - ck_lane(c)}")
+        else:
+            H[ck_lane(c)].insert(0, f"s_mov_b64 {LANE}, 1")
     for h in range(64):
         if X_FUSE and (h + 1) % 16:                          # a hop inside a row: R = -Fp (one of the two wait states), then the fused second fma
             H[h].insert(0, f"v_mov_b64 {R}, {cur['NFp']}")
@@ -222,9 +242,9 @@ def block(a, cur, nxt, tag):
     H = hop_fillers(cur, nxt)
     for j in range(BLOCK):
         lane, k = divmod(j, PER)
-        if j % 64 == 0 and X_CKPT and j % X_CKPT == 0:       # the state before every 64th symbol goes out: it sits in lane j / PER
-            a(f"v_readlane_b32 s46, {RLO}, {lane}")          # (R.hi is one instruction old: the read of R.lo is the wait state a v_readlane of a fresh result needs)
-            a(f"v_readlane_b32 s47, {RHI}, {lane}")
+        if j % 64 == 0 and j // 64 in CKPTS:                 # the state before every 64th symbol is kept: it sits in lane j / PER
+            a(f"v_cndmask_b32_e64 {CKLO}, {CKLO}, {RLO}, {LANE}")
+            a(f"v_cndmask_b32_e64 {CKHI}, {CKHI}, {RHI}, {LANE}")
         a(f"v_fma_f64 {T}, {R}, {cur['inv'][k]}, 1.0")
         if k < PER - 1:                                      # the lane's next symbol: in place
             a(f"v_fma_f64 {R}, {T}, {cur['F'][k]}, -{cur['F'][k]}")
@@ -237,6 +257,11 @@ def block(a, cur, nxt, tag):
                 a(f"v_mov_b32_dpp {T2LO}, {TLO} {DPP}")
                 a(f"v_fma_f64 {R}, {T2}, {cur['Fp']}, -{cur['Fp']}")
         a(f"v_and_or_b32 {RHI}, {RHI}, {MASK}, {EXPO}")
+    if CKPTS:                                                # the block's checkpoints go out together
+        a(f"s_mov_b64 exec, {CKLANES}")
+        a("s_nop 0")
+        a(f"global_store_dwordx2 {CKOFF}, {CKV}, {CK}")
+        a("s_mov_b64 exec, -1")
     a(f"s_add_u32 s44, s44, {8 * (BLOCK // 64)}")
     a("s_addc_u32 s45, s45, 0")
     a("s_sub_u32 s42, s42, 1")                               # blocks left, the one that starts now included
@@ -250,6 +275,7 @@ def body():
     a = Emitter()
     # operands: [rlo] [rhi] (v, in/out): the state - in: the same in every lane; out: valid in lane 0
     #           [blo] [bhi] (s): the records of the first block; [nblk] (s): blocks, >= 1; [clo] [chi] (s): where the first checkpoint goes
+    # every lane of the wave is active
     if X_ALIGN:
         a(".p2align 3")
     a(f"v_mov_b32 {RLO}, %[rlo]")
@@ -265,6 +291,17 @@ def body():
     a("s_addc_u32 s41, s37, 0")
     a(f"v_mbcnt_lo_u32_b32 {OFF}, -1, 0")
     a(f"v_mbcnt_hi_u32_b32 {OFF}, -1, {OFF}")
+    if CKPTS:
+        lanes = sum(1 << ck_lane(c) for c in CKPTS)
+        a(f"s_mov_b64 {LANE}, 1")
+        a(f"s_mov_b32 s48, 0x{lanes & 0xffffffff:x}")
+        a(f"s_mov_b32 s49, 0x{lanes >> 32:x}")
+        a(f"v_mul_u32_u24 {CKOFF}, {PER}, {OFF}")            # lane -> the first checkpoint at or behind its first symbol, 8 bytes each
+        a(f"v_add_u32 {CKOFF}, 63, {CKOFF}")
+        a(f"v_lshrrev_b32 {CKOFF}, 6, {CKOFF}")
+        a(f"v_lshlrev_b32 {CKOFF}, 3, {CKOFF}")
+        a(f"v_mov_b32 {CKLO}, 0")                            # (the other lanes' stay unused)
+        a(f"v_mov_b32 {CKHI}, 0")
     a(f"v_mul_u32_u24 {OFF}, {REC * PER}, {OFF}")
     a(f"v_mov_b32 {T2HI}, 0x3ff00000")                       # the high word of 1 + r * 2^-52
     a(f"v_mov_b32 {MASK}, 0x7fffff")

@@ -174,20 +174,17 @@ for j in range(64):
 add("m_none", "768 symbols with hops, no loads", body, 768, True)
 
 # ---- K: checkpoints ----
-for form, d in (("product", "s_nop 0, v_readlane x 2, s_nop 2, s_store_dwordx2 in front of every 64th symbol"), ("inhop", "the two v_readlane in a hop's wait states, the store after the hop"),
+for form, d in (("product", "two v_cndmask_b32 under a one-lane mask in front of every 64th symbol, the mask moved on in a hop's wait states, one store per block"),
                 ("none", "no checkpoints")):
-    body = []
+    body = ["s_mov_b64 s[56:57], 1", "s_nop 0"]
     for j in range(64):
-        if j % 5 == 0 and j // 5 < 12:
-            if form == "product":
-                body += ["s_nop 0", f"v_readlane_b32 s56, v{R}, {j}", f"v_readlane_b32 s57, v{R + 1}, {j}", "s_nop 2", f"s_store_dwordx2 s[56:57], s[58:59], 0x{8 * (j // 5):x}"]
-                body += lane_step(12, "product")
-            elif form == "inhop":
-                body += lane_step(12, "fill", [f"v_readlane_b32 s56, v{R}, {j}", f"v_readlane_b32 s57, v{R + 1}, {j}"]) + [f"s_store_dwordx2 s[56:57], s[58:59], 0x{8 * (j // 5):x}"]
-            else:
-                body += lane_step(12, "product")
+        if form == "product" and j % 5 == 0 and j // 5 < 12:
+            body += [f"v_cndmask_b32_e64 v38, v38, v{R}, s[56:57]", f"v_cndmask_b32_e64 v39, v39, v{R + 1}, s[56:57]"]
+            body += lane_step(12, "fill", ["s_lshl_b64 s[56:57], s[56:57], 5", "s_nop 0"])
         else:
             body += lane_step(12, "product")
+    if form == "product":
+        body += ["s_mov_b32 s64, 0x42108421", "s_mov_b32 s65, 0x00842108", "s_mov_b64 exec, s[64:65]", "global_store_dwordx2 v36, v[38:39], s[58:59]", "s_mov_b64 exec, -1"]
     add(f"k_{form}", f"768 symbols with hops, 12 checkpoints: {d}", body, 768, True)
 
 # ---- P: round 2 of this probe - the address of an 8-byte instruction (everything above runs wherever the prologue left the loop) ----

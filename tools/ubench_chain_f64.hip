@@ -65,8 +65,7 @@ __global__ void __launch_bounds__(64) k_chain_f64 (const uint8_t *recs, uint32_t
         d_step_f64 (R, C1[8], C1[9], C1[10], C1[11], c52); d_step_f64 (R, C1[12], C1[13], C1[14], C1[15], c52); \
     } while (0)
     for (uint32_t i = 0; i + 64 <= n; i += 64) {
-        if (ck) { const uint32_t lo = __builtin_amdgcn_readfirstlane (__double2loint (R)), hi = __builtin_amdgcn_readfirstlane (__double2hiint (R));
-                  asm volatile ("s_store_dwordx2 %0, %1, 0x0" : : "s"((uint64_t)lo | (uint64_t)hi << 32), "s"(ck + (size_t)blockIdx.x * (n / 32) + (i >> 5)) : "memory"); }
+        if (ck && !threadIdx.x) { uint32_t *c = ck + (size_t)blockIdx.x * (n / 32) + (i >> 5); c[0] = (uint32_t)__double2loint (R); c[1] = (uint32_t)__double2hiint (R); }
         HALF (a0, a1, b0, b1, 0); HALF (b0, b1, a0, a1, 1); HALF (a0, a1, b0, b1, 2); HALF (b0, b1, a0, a1, 3);
         HALF (a0, a1, b0, b1, 4); HALF (b0, b1, a0, a1, 5); HALF (a0, a1, b0, b1, 6); HALF (b0, b1, a0, a1, 7);
     }
@@ -89,7 +88,7 @@ __global__ void __launch_bounds__(64) k_chain_int (const uint8_t *recs, uint32_t
         d_step_int (range, C1[8], C1[9], C1[10], C1[11]); d_step_int (range, C1[12], C1[13], C1[14], C1[15]); \
     } while (0)
     for (uint32_t i = 0; i + 64 <= n; i += 64) {
-        if (ck) asm volatile ("s_store_dword %0, %1, 0x0" : : "s"(range), "s"(ck + (size_t)blockIdx.x * (n / 32) + (i >> 6)) : "memory");
+        if (ck && !threadIdx.x) ck[(size_t)blockIdx.x * (n / 32) + (i >> 6)] = range;
         HALF (a0, a1, b0, b1, 0); HALF (b0, b1, a0, a1, 1); HALF (a0, a1, b0, b1, 2); HALF (b0, b1, a0, a1, 3);
         HALF (a0, a1, b0, b1, 4); HALF (b0, b1, a0, a1, 5); HALF (a0, a1, b0, b1, 6); HALF (b0, b1, a0, a1, 7);
     }
@@ -128,7 +127,6 @@ template <int NOPS> __global__ void __launch_bounds__(64) k_chain_hop (const uin
         rlo = __builtin_amdgcn_readfirstlane (rlo); rhi = __builtin_amdgcn_readfirstlane (rhi);
         (void)done; (void)slow;
     }
-    asm volatile ("s_dcache_wb\n\ts_waitcnt lgkmcnt(0)" : : : "memory");
     const uint64_t t1 = __builtin_readcyclecounter (), w1 = wall_clock64 ();
     if (threadIdx.x == 0) { out[blockIdx.x] = __hiloint2double ((int)rhi, (int)rlo); if (cyc) { cyc[3 * blockIdx.x] = t1 - t0; cyc[3 * blockIdx.x + 1] = w1 - w0; cyc[3 * blockIdx.x + 2] = slow; } }
 }

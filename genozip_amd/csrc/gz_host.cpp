@@ -111,6 +111,14 @@ struct GzHandle {
     std::vector<ProfAcc> prof_view;        // gz_profile_get: this handle's totals + its helpers'
 };
 
+// a copy the host waits for, on the handle's own stream: one on the null stream can share a hardware queue with another handle's work - a long
+// chain, say - and would then wait behind it
+static hipError_t gz_copy (GzHandle *h, void *dst, const void *src, size_t n, hipMemcpyKind kind)
+{
+    const hipError_t e = hipMemcpyAsync (dst, src, n, kind, h->stream);
+    return e == hipSuccess ? hipStreamSynchronize (h->stream) : e;
+}
+
 static inline hipEvent_t gz_event_get (GzHandle *h)
 {
     if (!h->event_pool.empty ()) { hipEvent_t e = h->event_pool.back (); h->event_pool.pop_back (); return e; }
@@ -211,11 +219,11 @@ static GzHandle *gz_create_do (int device, void *hip_stream, int *err, bool back
     GzLogTable lt;
     for (int k = 0; k <= 256; k++) { lt.l10[k] = log (1024.0 + k); lt.l12[k] = log (4096.0 + k); }
     if (hipMalloc ((void **)&h->d_logs, sizeof (lt)) != hipSuccess ||
-        hipMemcpy (h->d_logs, &lt, sizeof (lt), hipMemcpyHostToDevice) != hipSuccess) {
+        gz_copy (h, h->d_logs, &lt, sizeof (lt), hipMemcpyHostToDevice) != hipSuccess) {
         if (h->own_stream) (void)hipStreamDestroy (h->stream);
         delete h; if (err) *err = GZ_ERR_HIP; return NULL;
     }
-    if (hipMalloc ((void **)&h->d_fail, 64) != hipSuccess || hipMemset (h->d_fail, 0, 64) != hipSuccess) { if (err) *err = GZ_ERR_HIP; gz_destroy (h); return NULL; }
+    if (hipMalloc ((void **)&h->d_fail, 64) != hipSuccess || hipMemsetAsync (h->d_fail, 0, 64, h->stream) != hipSuccess) { if (err) *err = GZ_ERR_HIP; gz_destroy (h); return NULL; }
     { const char *e = getenv ("GZ_NO_PIPELINE"); h->no_pipeline = e && *e && *e != '0'; }
     { const char *e = getenv ("GZ_MODEL_TILED"); h->tile_models = e && *e && *e != '0'; }
     { const char *e = getenv ("GZ_TM_DEBUG"); h->tm_dbg = e ? (uint32_t)atoi (e) : 0u; }
@@ -347,7 +355,7 @@ extern "C" int gz_download (GzHandle *h, void *dst, const void *src, uint64_t n)
     if (!h || (n && (!dst || !src))) return GZ_ERR_ARG;
     HIPCHK (h, hipSetDevice (h->device));
     HIPCHK (h, hipStreamSynchronize (h->stream));
-    if (n) HIPCHK (h, hipMemcpy (dst, src, n, hipMemcpyDeviceToHost));
+    if (n) HIPCHK (h, gz_copy (h, dst, src, n, hipMemcpyDeviceToHost));
     return GZ_OK;
 }
 
@@ -356,7 +364,7 @@ extern "C" int gz_upload (GzHandle *h, void *dst, const void *src, uint64_t n)
     if (!h || (n && (!dst || !src))) return GZ_ERR_ARG;
     HIPCHK (h, hipSetDevice (h->device));
     HIPCHK (h, hipStreamSynchronize (h->stream));
-    if (n) HIPCHK (h, hipMemcpy (dst, src, n, hipMemcpyHostToDevice));
+    if (n) HIPCHK (h, gz_copy (h, dst, src, n, hipMemcpyHostToDevice));
     return GZ_OK;
 }
 
@@ -1085,13 +1093,13 @@ static int gz_sync_do (GzHandle *h)
     bool device_failed = false;
     if (!h->pending.empty ()) {
         uint32_t f = 0;
-        HIPCHK (h, hipMemcpy (&f, h->d_fail, 4, hipMemcpyDeviceToHost));
-        if (f) { device_failed = true; HIPCHK (h, hipMemset (h->d_fail, 0, 4)); }
+        HIPCHK (h, gz_copy (h, &f, h->d_fail, 4, hipMemcpyDeviceToHost));
+        if (f) { device_failed = true; HIPCHK (h, hipMemsetAsync (h->d_fail, 0, 4, h->stream)); }
     }
     for (auto &pd : h->pending) {
         if (pd.kind == 0) {
             std::vector<GzdStream> S (pd.n_dev_streams);
-            HIPCHK (h, hipMemcpy (S.data (), pd.dev_streams, S.size () * sizeof (GzdStream), hipMemcpyDeviceToHost));
+            HIPCHK (h, gz_copy (h, S.data (), pd.dev_streams, S.size () * sizeof (GzdStream), hipMemcpyDeviceToHost));
             GzStream *u = (GzStream *)pd.user;
             for (int i = 0; i < pd.n; i++) {
                 if (u[i].status != GZ_ST_PENDING) continue;
@@ -1101,7 +1109,7 @@ static int gz_sync_do (GzHandle *h)
         }
         else if (pd.kind == 1) {
             std::vector<GzdDecStream> S (pd.n_dev_streams);
-            HIPCHK (h, hipMemcpy (S.data (), pd.dev_streams, S.size () * sizeof (GzdDecStream), hipMemcpyDeviceToHost));
+            HIPCHK (h, gz_copy (h, S.data (), pd.dev_streams, S.size () * sizeof (GzdDecStream), hipMemcpyDeviceToHost));
             GzStream *u = (GzStream *)pd.user;
             for (int i = 0; i < pd.n; i++) {
                 if (u[i].status != GZ_ST_PENDING) continue;
@@ -1111,7 +1119,7 @@ static int gz_sync_do (GzHandle *h)
         }
         else {
             std::vector<GzdVB> V (pd.n);
-            HIPCHK (h, hipMemcpy (V.data (), pd.dev_vbs, V.size () * sizeof (GzdVB), hipMemcpyDeviceToHost));
+            HIPCHK (h, gz_copy (h, V.data (), pd.dev_vbs, V.size () * sizeof (GzdVB), hipMemcpyDeviceToHost));
             GzVBlock *u = (GzVBlock *)pd.user;
             for (int i = 0; i < pd.n; i++) {
                 u[i].status = V[i].status == GZ_ST_OK ? GZ_OK : V[i].status == GZ_ST_TOO_SMALL ? GZ_TOO_SMALL : GZ_ERR;
@@ -1180,7 +1188,7 @@ extern "C" int gz_codec_compress_host (GzHandle *h, int codec, const uint8_t *in
     const int rc2 = gz_sync (h);                      // (also when the batch call failed: nothing stays pending)
     if (rc == GZ_OK && rc2 < 0) rc = rc2;
     if (rc == GZ_OK && s.status != GZ_OK) rc = s.status;
-    if (rc == GZ_OK && s.out_len && (e = hipMemcpy (out, d_out, s.out_len, hipMemcpyDeviceToHost)) != hipSuccess) {
+    if (rc == GZ_OK && s.out_len && (e = gz_copy (h, out, d_out, s.out_len, hipMemcpyDeviceToHost)) != hipSuccess) {
         h->err = std::string ("hipMemcpy: ") + hipGetErrorString (e); rc = GZ_ERR_HIP;
     }
     (void)hipFree (d_buf);
@@ -1227,7 +1235,7 @@ extern "C" int gz_codec_uncompress_host (GzHandle *h, int codec, const uint8_t *
     if ((rc = gz_codec_uncompress_batch (h, &s, 1)) != GZ_OK) return rc;
     if ((rc = gz_sync (h)) < 0) return rc;
     if (s.status != GZ_OK) return s.status;
-    if (out_len) HIPCHK (h, hipMemcpy (out, d_out, out_len, hipMemcpyDeviceToHost));
+    if (out_len) HIPCHK (h, gz_copy (h, out, d_out, out_len, hipMemcpyDeviceToHost));
     return GZ_OK;
 }
 
@@ -1401,7 +1409,7 @@ extern "C" int gz_codec_assign_best_host (GzHandle *h, const uint8_t *in, uint32
     uint8_t *d = NULL;
     HIPCHK (h, hipSetDevice (h->device));
     HIPCHK (h, hipMalloc ((void **)&d, (size_t)in_len + 16));
-    int rc = hipMemcpy (d, in, in_len, hipMemcpyHostToDevice) == hipSuccess ? gz_codec_assign_best (h, d, in_len, NULL) : GZ_ERR_HIP;
+    int rc = gz_copy (h, d, in, in_len, hipMemcpyHostToDevice) == hipSuccess ? gz_codec_assign_best (h, d, in_len, NULL) : GZ_ERR_HIP;
     (void)hipFree (d);
     return rc;
 }
@@ -1560,7 +1568,7 @@ static int local_partial (GzHandle *h, int ltype, void *data, uint64_t n_present
     P.missing = missing; P.miss_t = miss_t; P.cells = cells; P.rows = rows; P.cols = cols; P.w = w; P.n_present = n_present;
     P.in = (const uint8_t *)data; P.out = (uint8_t *)scratch; P.to_file = to_file ? 1 : 0;
     const int32_t ok = GZ_ST_OK;
-    HIPCHK (h, hipMemcpy (P.status, &ok, 4, hipMemcpyHostToDevice));
+    HIPCHK (h, gz_copy (h, P.status, &ok, 4, hipMemcpyHostToDevice));
     hipLaunchKernelGGL (k_transpose, dim3 ((cols + 31) / 32, (rows + 31) / 32), dim3 (32, 8), 32 * 33 * 4 + 128, h->stream, missing, miss_t, rows, cols, 1u);
     KLAUNCH (h, k_ptr_count, dim3 (tiles, 2), dim3 (256), 2048, P);
     KLAUNCH (h, k_ptr_scan, dim3 (2), dim3 (256), 2048, P);
@@ -1574,7 +1582,7 @@ static int local_partial (GzHandle *h, int ltype, void *data, uint64_t n_present
     HIPCHK (h, hipGetLastError ());
     HIPCHK (h, hipStreamSynchronize (h->stream));
     int32_t st = 0;
-    HIPCHK (h, hipMemcpy (&st, P.status, 4, hipMemcpyDeviceToHost));
+    HIPCHK (h, gz_copy (h, &st, P.status, 4, hipMemcpyDeviceToHost));
     if ((rc = gz_sync (h)) < 0) return rc;
     if (st != GZ_ST_OK) { h->err = "partial transpose: the mask does not leave n_present elements"; return GZ_ERR_CORRUPT; }
     if (!to_file) return base;
@@ -1597,7 +1605,7 @@ extern "C" int gz_adler32 (GzHandle *h, const uint8_t *data, uint64_t len, uint3
     hipLaunchKernelGGL (k_adler32, dim3 (1), dim3 (256), 4096, h->stream, data, (uint32_t)len, d);
     HIPCHK (h, hipGetLastError ());
     HIPCHK (h, hipStreamSynchronize (h->stream));
-    HIPCHK (h, hipMemcpy (adler_out, d, 4, hipMemcpyDeviceToHost));
+    HIPCHK (h, gz_copy (h, adler_out, d, 4, hipMemcpyDeviceToHost));
     return GZ_OK;
 }
 
@@ -1623,7 +1631,7 @@ extern "C" int gz_acgt_pack (GzHandle *h, const uint8_t *seq, uint64_t n_bases, 
     HIPCHK (h, hipGetLastError ());
     HIPCHK (h, hipStreamSynchronize (h->stream));
     uint32_t f = 0;
-    HIPCHK (h, hipMemcpy (&f, d, 4, hipMemcpyDeviceToHost));
+    HIPCHK (h, gz_copy (h, &f, d, 4, hipMemcpyDeviceToHost));
     *has_x_host = f != 0;
     return gz_sync (h) < 0 ? GZ_ERR : GZ_OK;
 }
@@ -1918,8 +1926,8 @@ extern "C" int gz_vb_uncompress_many (GzHandle *h, int n_vbs, const uint8_t *con
     HIPCHK (h, hipGetLastError ());
     HIPCHK (h, hipStreamSynchronize (h->stream));
     std::vector<GzdVbSec> S (n_secs);
-    HIPCHK (h, hipMemcpy (W.data (), d_w, W.size () * sizeof (GzdVbWalk), hipMemcpyDeviceToHost));
-    HIPCHK (h, hipMemcpy (S.data (), d_s, n_secs * sizeof (GzdVbSec), hipMemcpyDeviceToHost));
+    HIPCHK (h, gz_copy (h, W.data (), d_w, W.size () * sizeof (GzdVbWalk), hipMemcpyDeviceToHost));
+    HIPCHK (h, gz_copy (h, S.data (), d_s, n_secs * sizeof (GzdVbSec), hipMemcpyDeviceToHost));
     std::vector<GzStream> work;
     for (int v = 0; v < n_vbs; v++) {
         if (W[v].status != GZ_ST_OK) { h->err = "bad VB header / section magic / section overflow"; return GZ_ERR_CORRUPT; }

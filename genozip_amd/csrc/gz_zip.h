@@ -462,7 +462,7 @@ static int zip_pick_codec (GzHandle *h, GzZipFile *f, const uint8_t dict_id[8], 
     GzCodecTest extra[8]; int n_extra = 0;
     if (f->hostc.trial) {
         std::vector<uint8_t> host (sample);
-        HIPCHK (h, hipMemcpy (host.data (), in, sample, hipMemcpyDeviceToHost));
+        HIPCHK (h, gz_copy (h, host.data (), in, sample, hipMemcpyDeviceToHost));
         n_extra = f->hostc.trial (f->hostc.user, dict_id, is_local, host.data (), sample, extra, 8);
         if (n_extra < 0 || n_extra > 8) { h->err = "host codec trial"; return GZ_ERR; }
         for (int i = 0; i < n_extra; i++) {
@@ -1166,6 +1166,8 @@ extern "C" int gz_fastq_zip_seg (GzZipFile *f, uint8_t *text, uint64_t text_len,
         if ((int32_t)icolres[2 * k + 1] == GZ_ST_CORRUPT) { h->err = "an ordered item is not an integer (qname.c:750-756)"; ZIP_FAIL (GZ_ERR_CORRUPT); }
     for (size_t k = 0; k < NCJ; k++) if (K.colres[k].status != 1) { h->err = "column dictionary capacity"; ZIP_FAIL (GZ_ERR); }
     if (!pack_total[1]) { h->err = "merge staging buffer too small"; ZIP_FAIL (GZ_ERR); }
+    f->stage.resize (pack_total[0] + 16);
+    if (pack_total[0] && gz_copy (h, f->stage.data (), d_staging, pack_total[0], hipMemcpyDeviceToHost) != hipSuccess) { h->err = "copy (merge staging)"; ZIP_FAIL (GZ_ERR_HIP); }
     // speculation: this file's own trial, on the main handle - idle now until the merge (host) has the dictionaries - and only of
     // the form of QUAL the file uses; its sizes are read in the merge phase, with the other trial compressions'
     if (!K.spec_trial.empty () && qmode >= 0 && COL (0, (uint32_t)f->qual_ctx).local_len >= 50) {     // (codec.c:311-312: too small a sample decides nothing)
@@ -1174,8 +1176,6 @@ extern "C" int gz_fastq_zip_seg (GzZipFile *f, uint8_t *text, uint64_t text_len,
             K.spec_pending = true; K.spec_t = t;
         }
     }
-    f->stage.resize (pack_total[0] + 16);
-    if (pack_total[0] && hipMemcpy (f->stage.data (), d_staging, pack_total[0], hipMemcpyDeviceToHost) != hipSuccess) { h->err = "hipMemcpy (merge staging)"; ZIP_FAIL (GZ_ERR_HIP); }
 
     // ---- the merge blob: per VBlock, per context, what ctx_merge_in_one_vctx reads of the VBlock's context ------------------
     K.blob.clear ();

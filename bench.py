@@ -1097,13 +1097,13 @@ def main():
     alg_per_launch = alg_bytes_per_step / per_step_launches
     achieved = alg_per_launch / (max(avg_launch_ms, 1e-6) / 1e3) / 1e9
     tr = pmc_traffic(dom, a)
-    # The critical path. The dominant kernel is launched several times per step on different streams (the persistent launch over the long
-    # QUAL streams + the short-leaf launches of trials and section writer): its launches overlap, their sum is NOT time on the step's
-    # critical path - the LONGEST launch is. That launch codes the long streams (sections of >= 1 MB); what bounds it is the issue rate
+    # The critical path. The dominant kernel is launched several times per step on different streams (the batch over the long
+    # QUAL streams + the short-leaf launches of trials and section writer): they overlap, their sum is NOT time on the step's
+    # critical path - the LONGEST is (a batch's chunk launches count as one: gz_profile). That one codes the long streams (sections of >= 1 MB); what bounds it is the issue rate
     # of one wave per stream, not HBM: three dependent vector instructions per symbol (12.07 clocks = 5.03 ns at 2.4 GHz: the floor) + a
     # lane hop every 16 symbols, the checkpoints and the operand loads in the hops' wait states = 13.00 clocks = 5.41 ns with the loop alone
     # on the device (tools/ubench_chain_f64.hip; round 5: 15.1, round 4: 15.8, rounds 1-3: seven scalar integer instructions, 12.7 ns).
-    # ns_per_symbol below is the whole launch / the symbols of its longest stream: it includes the wait for the first chunk's models.
+    # ns_per_symbol below is the time from its first launch to the end of its last / the symbols of its longest stream.
     secs_all = [s for z in z_all for s in walk_sections(z)]
     long_secs = [s for s in secs_all if s[3] >= (1 << 20) and s[1] in (16, 17, 18, 19)]
     longest_ms = prof_max.get(dom, avg_launch_ms)

@@ -46,42 +46,34 @@ struct Pending {          // results to hand back at gz_sync()
 
 struct ArenaBlock { uint8_t *base; size_t size, used; };
 
-// More hardware queues than the HIP runtime's default of 4 (see genozip_amd/lib.py, INTEGRATION.md): only effective when this library is
+// More hardware queues than the HIP runtime's default of 4 (see genozip_amd/lib.py): only effective when this library is
 // loaded before the process's first HIP call; never overrides what the host has set.
 __attribute__((constructor)) static void gz_runtime_env (void) { setenv ("GPU_MAX_HW_QUEUES", "8", 0); }
-
-// workgroups of persistent chain kernels in flight in this process / those of them that hold a whole compute unit
-static std::atomic<int> g_chain_wgs (0), g_chain_cus (0);
 
 #define GZ_MAX_CHUNKS 129    // position chunks of the arithmetic coder's pipeline: at most 16 - or GZ_ARITH_CHUNKS - (arith_pipe_setup) + a partial one
 struct GzHandle {
     int device;
     hipStream_t stream;
-    hipStream_t stream2;      // side stream: work that is independent of the arithmetic coder's long chain runs beside it
-    hipEvent_t ev_fork, ev_join;
-    hipStream_t stream3;      // the range coder chain of position chunk k runs here, beside the models of chunk k+1
-    hipStream_t stream4;      // the models: like stream2 kept off the compute units reserved for the chain
-    hipEvent_t ev_model_fork;
-    hipStream_t stream5;      // model + chain of the leaves that fit one chunk
-    hipEvent_t ev_small;
-    hipStream_t stream6;      // the `low` kernels of the long leaves, following the chain chunk by chunk
-    hipEvent_t ev_low;
-    hipStream_t stream7;      // the context sort of position chunk k+1, beside the models of chunk k
-    hipEvent_t ev_sort[GZ_MAX_CHUNKS];
-    hipEvent_t ev_chain_go, ev_chain;   // the persistent chain may start / has finished
+    // Few streams: the runtime maps a process's streams onto GPU_MAX_HW_QUEUES hardware queues (a new stream joins the queue with the fewest, the
+    // youngest of those), and what shares a queue runs in the order it was queued. With 8 queues the VBlock driver's pair of handles has one per
+    // stream; with 4 the order of creation - a background handle's three at once, `aux` before `side`, an ordinary handle's `aux` when it is
+    // first needed - keeps the long chain's queue free of what the call waits for.
+    hipStream_t side;         // the short arithmetic leaves, and the range coder's chain of the long ones
+    hipStream_t aux = NULL;   // the rANS leaves, and the `low` kernels of the long arithmetic ones
+    hipEvent_t ev_fork, ev_join, ev_events;
+    hipEvent_t ev_model[GZ_MAX_CHUNKS], ev_chain[GZ_MAX_CHUNKS];   // position chunk k: its records are there / its checkpoints are
     int n_cu = 0;             // compute units of the device
-    int chain_wgs_held = 0, chain_cus_held = 0;   // this handle's share of g_chain_wgs / g_chain_cus, returned at gz_sync
-    uint32_t *d_fail = NULL;  // set by a kernel that gave up (the persistent chain when the models never report)
+    uint32_t *d_fail = NULL;  // set by a kernel that gave up (the chain of a position chunk whose records were not announced)
     GzHandle *emit_after = NULL;   // the next VBlock batch's section writer waits for this handle's queued work (gz_emit_after)
     GzHandle *emit_after_used = NULL;   // what the batch being queued right now has consumed of it
     hipEvent_t ev_other = NULL;
     std::string warn;         // gz_last_warning: a call that succeeded has something to say (the chain fallback)
     uint32_t tm_dbg = 0;
     bool tile_models = false; // GZ_MODEL_TILED=1: the leaves of small alphabets through k_arith_model_tiled (one workgroup per leaf, records leave coalesced) - exact, less traffic, SLOWER: off
-    bool no_pipeline = false; // GZ_NO_PIPELINE=1: no persistent kernel (needed under tools that serialise kernels, e.g. rocprofv3 --pmc)
-    bool in_fallback = false; // gz_sync is running a batch again, unpipelined, after its persistent chain never heard from the models
+    bool no_pipeline = false; // GZ_NO_PIPELINE=1: every leaf in one piece, one stream
+    bool in_fallback = false; // gz_sync is running a batch again, unpipelined, after its chain did not find the models' records
     uint32_t chain_fallbacks = 0;           // how often that has happened on this handle (gz_chain_fallbacks)
-    bool debug_starve_chain = false;        // GZ_DEBUG_STARVE_CHAIN=1 (tests): the models' progress is never announced - the chain must time out, the batch must still come out right
+    bool debug_starve_chain = false;        // GZ_DEBUG_STARVE_CHAIN=1 (tests): the models' progress is never announced - the chain must notice, the batch must still come out right
     bool own_stream;
     std::vector<ArenaBlock> blocks;
     std::vector<Pending> pending;
@@ -171,8 +163,7 @@ extern "C" const char *gz_version (void) { return GZ_VERSION; }
 
 static GzHandle *gz_create_do (int device, void *hip_stream, int *err, bool background);
 extern "C" GzHandle *gz_create (int device, void *hip_stream, int *err) { return gz_create_do (device, hip_stream, err, false); }
-// a handle for long-running work that must not hold up another handle's short kernels: all its streams but the chain's at the
-// lowest priority (the VBlock compute driver codes the long QUAL streams on such a handle)
+// a handle for long-running work beside another handle's short kernels (the VBlock compute driver codes the long QUAL streams on such a handle)
 extern "C" GzHandle *gz_create_background (int device, int *err) { return gz_create_do (device, NULL, err, true); }
 
 static GzHandle *gz_create_do (int device, void *hip_stream, int *err, bool background)
@@ -186,35 +177,22 @@ static GzHandle *gz_create_do (int device, void *hip_stream, int *err, bool back
     GzHandle *h = new GzHandle ();
     h->device = device; h->d_logs = NULL; h->background = background;
     h->arena_block_size = (size_t)256 << 20;
-    int prio_lo0 = 0, prio_hi0 = 0;
-    if (hipDeviceGetStreamPriorityRange (&prio_lo0, &prio_hi0) != hipSuccess) prio_lo0 = prio_hi0 = 0;
     if (hip_stream) { h->stream = (hipStream_t)hip_stream; h->own_stream = false; }
     else {
-        if (hipStreamCreateWithPriority (&h->stream, hipStreamNonBlocking, background ? prio_lo0 : (prio_lo0 + prio_hi0) / 2) != hipSuccess) { delete h; if (err) *err = GZ_ERR_HIP; return NULL; }
+        if (hipStreamCreateWithFlags (&h->stream, hipStreamNonBlocking) != hipSuccess) { delete h; if (err) *err = GZ_ERR_HIP; return NULL; }
         h->own_stream = true;
     }
-    // The chain (one wave per leaf, strictly serial) is the critical path: its few workgroups must not queue behind
-    // the tens of thousands of the model kernel launched at the same moment, so its stream gets the highest priority and
-    // the streams of the kernels that run beside it the lowest.
     if (hipDeviceGetAttribute (&h->n_cu, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || h->n_cu <= 0) h->n_cu = 64;
-    int prio_lo = 0, prio_hi = 0;
-    if (hipDeviceGetStreamPriorityRange (&prio_lo, &prio_hi) != hipSuccess) prio_lo = prio_hi = 0;
-    if (!background) prio_lo = (prio_lo + prio_hi) / 2;      // an ordinary handle's side streams: the middle; a background handle's: the lowest
-    if (hipStreamCreateWithPriority (&h->stream2, hipStreamNonBlocking, prio_lo) != hipSuccess ||
-        hipStreamCreateWithPriority (&h->stream3, hipStreamNonBlocking, prio_hi) != hipSuccess ||
-        hipStreamCreateWithPriority (&h->stream4, hipStreamNonBlocking, prio_lo) != hipSuccess ||
-        hipStreamCreateWithPriority (&h->stream5, hipStreamNonBlocking, prio_lo) != hipSuccess ||
-        hipStreamCreateWithPriority (&h->stream6, hipStreamNonBlocking, prio_lo) != hipSuccess ||
-        hipStreamCreateWithPriority (&h->stream7, hipStreamNonBlocking, prio_lo) != hipSuccess ||
-        hipEventCreateWithFlags (&h->ev_low, hipEventDisableTiming) != hipSuccess ||
-        hipEventCreateWithFlags (&h->ev_small, hipEventDisableTiming) != hipSuccess ||
-        hipEventCreateWithFlags (&h->ev_model_fork, hipEventDisableTiming) != hipSuccess ||
-        hipEventCreateWithFlags (&h->ev_chain, hipEventDisableTiming) != hipSuccess ||
-        hipEventCreateWithFlags (&h->ev_chain_go, hipEventDisableTiming) != hipSuccess ||
+    // (all streams at the default priority: the order between them is the events' alone)
+    if ((background && hipStreamCreateWithFlags (&h->aux, hipStreamNonBlocking) != hipSuccess) ||
+        hipStreamCreateWithFlags (&h->side, hipStreamNonBlocking) != hipSuccess ||
+        hipEventCreateWithFlags (&h->ev_events, hipEventDisableTiming) != hipSuccess ||
         hipEventCreateWithFlags (&h->ev_fork, hipEventDisableTiming) != hipSuccess ||
         hipEventCreateWithFlags (&h->ev_join, hipEventDisableTiming) != hipSuccess) { delete h; if (err) *err = GZ_ERR_HIP; return NULL; }
     for (int k = 0; k < GZ_MAX_CHUNKS; k++)
-        if (hipEventCreateWithFlags (&h->ev_sort[k], hipEventDisableTiming) != hipSuccess) { delete h; if (err) *err = GZ_ERR_HIP; return NULL; }
+        if (hipEventCreateWithFlags (&h->ev_model[k], hipEventDisableTiming) != hipSuccess || hipEventCreateWithFlags (&h->ev_chain[k], hipEventDisableTiming) != hipSuccess) {
+            delete h; if (err) *err = GZ_ERR_HIP; return NULL;
+        }
     // log(1024+k), log(4096+k) from the host libm: what the reference's compute_shift() sees (rANS_static4x16pr.c:647)
     GzLogTable lt;
     for (int k = 0; k <= 256; k++) { lt.l10[k] = log (1024.0 + k); lt.l12[k] = log (4096.0 + k); }
@@ -245,7 +223,6 @@ static void prof_collect (GzHandle *h);
 
 extern "C" void gz_destroy (GzHandle *h)
 {
-    if (h) { g_chain_wgs.fetch_sub (h->chain_wgs_held); g_chain_cus.fetch_sub (h->chain_cus_held); h->chain_wgs_held = h->chain_cus_held = 0; }
     if (!h) return;
     (void)hipSetDevice (h->device);
     (void)hipStreamSynchronize (h->stream);
@@ -256,19 +233,10 @@ extern "C" void gz_destroy (GzHandle *h)
     (void)hipFree (h->d_logs);
     (void)hipFree (h->d_fail);
     if (h->own_stream) (void)hipStreamDestroy (h->stream);
-    (void)hipStreamDestroy (h->stream2);
-    (void)hipStreamDestroy (h->stream3);
-    (void)hipStreamDestroy (h->stream4);
-    (void)hipStreamDestroy (h->stream5);
-    (void)hipStreamDestroy (h->stream6);
-    (void)hipStreamDestroy (h->stream7);
-    for (int k = 0; k < GZ_MAX_CHUNKS; k++) (void)hipEventDestroy (h->ev_sort[k]);
-    (void)hipEventDestroy (h->ev_low);
-    (void)hipEventDestroy (h->ev_small);
-    (void)hipEventDestroy (h->ev_model_fork);
-    (void)hipEventDestroy (h->ev_chain);
-    (void)hipEventDestroy (h->ev_chain_go);
-    (void)hipEventDestroy (h->ev_fork); (void)hipEventDestroy (h->ev_join);
+    (void)hipStreamDestroy (h->side);
+    if (h->aux) (void)hipStreamDestroy (h->aux);
+    for (int k = 0; k < GZ_MAX_CHUNKS; k++) { (void)hipEventDestroy (h->ev_model[k]); (void)hipEventDestroy (h->ev_chain[k]); }
+    (void)hipEventDestroy (h->ev_fork); (void)hipEventDestroy (h->ev_join); (void)hipEventDestroy (h->ev_events);
     if (h->ev_other) (void)hipEventDestroy (h->ev_other);
     delete h;
 }
@@ -562,7 +530,10 @@ static int upload (GzHandle *h, const void *host, size_t bytes, void **dev)
     return GZ_OK;
 }
 
-// kernels that run beside the pipelined chain ask for this much LDS so that they never fit on a chain's compute unit
+// The chain's workgroups ask for (nearly) the whole LDS of a compute unit although they use none, so that no workgroup of another kernel that
+// needs LDS fits beside them: the chain waves are the critical path of the step and share instruction fetch and issue with nobody (default step
+// without: 47 instead of 39 ms). Kernels that run beside them ask for more than what that leaves.
+#define GZ_CHAIN_LDS (156 * 1024)
 #define GZ_KEEP_OFF_LDS 4608                  // (the chain leaves 4096 bytes of a compute unit free)
 // the decoder's models by LDS need (gz_kernels_dec.h: a literal row is 128 words per 64 entries): order 0 - 16 KB; order 1 up to 64 symbols
 // - 42.5 KB, three to a compute unit; up to 80 symbols (quality scores) - 80 KB, two to a compute unit; up to 128 - 140 KB; beyond: global memory
@@ -574,10 +545,9 @@ struct ArithPipe {
     uint32_t np = 0, no1 = 0, nlb = 0, nlb_small = 0, nbig = 0, nsmall = 0, chunk = 0, n_chunks = 1;
     const uint32_t *d_plain = NULL, *d_o1 = NULL, *d_big = NULL, *d_small = NULL, *d_rle = NULL;
     const GzdLowBlock *d_lb = NULL, *d_lb_small = NULL;
-    uint32_t *d_progress = NULL;      // [0] model chunks announced  [16 + k] leaves whose chain is through chunk k
-    uint32_t *d_bounds = NULL;        // [n_chunks + 1] where the position chunks start (device copy of bounds)
+    uint32_t *d_progress = NULL;      // model chunks announced
     std::vector<uint32_t> bounds;     // the first chunk of `chunk` positions goes in pieces: 1/8, 1/8, 1/4, 1/2 of it (whole sort tiles)
-    bool pipelined = false, reserve_cu = false;
+    bool pipelined = false;
 };
 
 static int arith_pipe_setup (GzHandle *h, Plan &P, ArithPipe &A)
@@ -633,24 +603,10 @@ static int arith_pipe_setup (GzHandle *h, Plan &P, ArithPipe &A)
     std::vector<uint32_t> big, small;
     for (size_t i = 0; i < P.plain_list.size (); i++) (P.plain_nb[i] > A.chunk ? big : small).push_back (P.plain_list[i]);
     A.nbig = (uint32_t)big.size (); A.nsmall = (uint32_t)small.size ();
-    // The persistent chain waits (on the device) for the models, so it must never keep them from running: all its
-    // workgroups are resident at once, and they may take at most half the wave slots of the device (4 waves each,
-    // 32 slots per compute unit). More long leaves than that: no pipeline, everything in one piece (correct, slower).
-    const uint32_t chain_wgs = (A.nbig + GZ_CHAIN_WAVES - 1) / GZ_CHAIN_WAVES;
-    // (the budget is per process: several handles - one per host thread, INTEGRATION.md - share the device)
-    A.pipelined = false; A.reserve_cu = false;
     // (on a background handle a batch whose longest leaf is under two chunks - the 99 999-byte sample of the QUAL trial, which sits in
-    //  front of the long pole - goes in one piece: 6.5 -> 4.5 ms, it gains nothing from the pipeline and pays for its gates. The same
+    //  front of the long pole - goes in one piece: 6.5 -> 4.5 ms, it gains nothing from the pipeline and pays for its launches. The same
     //  rule on the main handle made the step 9 ms SLOWER: its trial batches then hold up the sections that run beside the long pole)
-    if (A.nbig && !h->no_pipeline && !h->in_fallback && (!h->background || P.max_arith_n > 2 * GZ_CHUNK_MIN)) {
-        const int wgs = (int)chain_wgs;
-        if (g_chain_wgs.fetch_add (wgs) + wgs <= h->n_cu * 4) {
-            A.pipelined = true; h->chain_wgs_held += wgs;
-            if (g_chain_cus.fetch_add (wgs) + wgs <= h->n_cu / 4) { A.reserve_cu = true; h->chain_cus_held += wgs; }   // a whole compute unit each only while that leaves 3/4 to the rest
-            else g_chain_cus.fetch_sub (wgs);
-        }
-        else g_chain_wgs.fetch_sub (wgs);
-    }
+    A.pipelined = A.nbig && !h->no_pipeline && !h->in_fallback && (!h->background || P.max_arith_n > 2 * GZ_CHUNK_MIN);
     if (!A.pipelined) { A.nbig = 0; small = P.plain_list; big.clear (); A.nsmall = (uint32_t)small.size (); }
     if (getenv ("GZ_DEBUG_PIPE")) {
         uint64_t sum_big = 0; uint32_t mx = 0, mn = 0xffffffffu;
@@ -669,8 +625,8 @@ static int arith_pipe_setup (GzHandle *h, Plan &P, ArithPipe &A)
                 fprintf (stderr, "[list] %s %zu: codec %u method 0x%02x plane %u stream %u in_len %u\n", pass ? "small" : "big", i, P.streams[L.stream].codec_req, L.method, L.plane, L.stream, P.streams[L.stream].in_len); }
         }
 #endif
-        fprintf (stderr, "[pipe] bg %d np %u nbig %u nsmall %u max_arith_n %u chunk %u n_chunks %u pipelined %d reserve %d big: min %u max %u sum %llu\n", (int)h->background, A.np, A.nbig, A.nsmall,
-                 P.max_arith_n, A.chunk, A.n_chunks, (int)A.pipelined, (int)A.reserve_cu, mn, mx, (unsigned long long)sum_big);
+        fprintf (stderr, "[pipe] bg %d np %u nbig %u nsmall %u max_arith_n %u chunk %u n_chunks %u pipelined %d big: min %u max %u sum %llu\n", (int)h->background, A.np, A.nbig, A.nsmall,
+                 P.max_arith_n, A.chunk, A.n_chunks, (int)A.pipelined, mn, mx, (unsigned long long)sum_big);
     }
     void *d;
     int rc = upload (h, P.plain_list.data (), P.plain_list.size () * 4, &d); A.d_plain = (const uint32_t *)d;
@@ -681,9 +637,8 @@ static int arith_pipe_setup (GzHandle *h, Plan &P, ArithPipe &A)
     if (rc != GZ_OK) return rc;
     if (A.pipelined) {
         if (A.n_chunks > GZ_MAX_CHUNKS) return GZ_ERR;            // (cannot happen: at most 16 / GZ_ARITH_CHUNKS chunks)
-        if (!(A.d_progress = (uint32_t *)arena_alloc (h, 1024))) return GZ_ERR_HIP;
-        HIPCHK (h, hipMemsetAsync (A.d_progress, 0, 1024, h->stream));
-        { void *db; if ((rc = upload (h, A.bounds.data (), A.bounds.size () * 4, &db)) != GZ_OK) return rc; A.d_bounds = (uint32_t *)db; }
+        if (!(A.d_progress = (uint32_t *)arena_alloc (h, 64))) return GZ_ERR_HIP;
+        HIPCHK (h, hipMemsetAsync (A.d_progress, 0, 64, h->stream));
         if (A.nsmall) {                                           // the slices of the short leaves only
             std::vector<uint8_t> is_small (P.leaves.size (), 0);
             for (uint32_t l : small) is_small[l] = 1;
@@ -697,17 +652,6 @@ static int arith_pipe_setup (GzHandle *h, Plan &P, ArithPipe &A)
     return GZ_OK;
 }
 
-// the persistent chain of the long leaves: launched before everything else so that it finds free compute units
-static int arith_launch_chain (GzHandle *h, const ArithPipe &A, GzdLeaf *d_leaves)
-{
-    HIPCHK (h, hipEventRecord (h->ev_chain_go, h->stream));                     // (behind the uploads and the memset)
-    HIPCHK (h, hipStreamWaitEvent (h->stream3, h->ev_chain_go, 0));
-    KLAUNCH_ON (h, h->stream3, k_arith_chain, dim3 ((A.nbig + GZ_CHAIN_WAVES - 1) / GZ_CHAIN_WAVES), dim3 (64 * GZ_CHAIN_WAVES), A.reserve_cu ? GZ_CHAIN_LDS : 64,
-                d_leaves, A.d_big, A.nbig, (const uint32_t *)A.d_progress, (const uint32_t *)A.d_bounds, h->d_fail, A.d_progress + 16, A.n_chunks);
-    HIPCHK (h, hipEventRecord (h->ev_chain, h->stream3));
-    return GZ_OK;
-}
-
 static int launch_encode (GzHandle *h, Plan &P, GzdStream *d_streams, GzdLeaf *d_leaves, GzdVB *d_vbs, uint32_t n_vbs, int section_mode)
 {
     const uint32_t ns = (uint32_t)P.streams.size (), nl = (uint32_t)P.leaves.size ();
@@ -715,9 +659,6 @@ static int launch_encode (GzHandle *h, Plan &P, GzdStream *d_streams, GzdLeaf *d
     ArithPipe A;
     int rc = arith_pipe_setup (h, P, A);
     if (rc != GZ_OK) return rc;
-#ifndef GZ_SEQUENTIAL_STREAMS
-    if (A.pipelined && (rc = arith_launch_chain (h, A, d_leaves)) != GZ_OK) return rc;
-#endif
     KLAUNCH (h, k_resolve, dim3 ((ns + 255) / 256), dim3 (256), 0, d_streams, ns, section_mode);
     if (P.any_striped) {
         uint32_t chunks = (P.max_in / 16 + 255) / 256;
@@ -728,15 +669,15 @@ static int launch_encode (GzHandle *h, Plan &P, GzdStream *d_streams, GzdLeaf *d
     if (nl) {
         KLAUNCH (h, k_presence, dim3 (nl, GZ_PRES_SLICES), dim3 (256), 1024, d_streams, d_leaves);
         KLAUNCH (h, k_leaf_prep, dim3 (nl), dim3 (256), 4096, d_streams, d_leaves);
-        // fork: the rANS leaves and the run-length arith leaves do not depend on the model/chain kernels of the plain
-        // arith leaves, so they run beside them on a second stream
+        // fork: the rANS leaves do not depend on the kernels of the arithmetic leaves, so they run beside them on a second stream
         const bool fork = P.any_arith;
-        hipStream_t side = fork ? h->stream2 : h->stream;
-        if (fork) { HIPCHK (h, hipEventRecord (h->ev_fork, h->stream)); HIPCHK (h, hipStreamWaitEvent (side, h->ev_fork, 0)); }
+        if (fork && !h->aux) HIPCHK (h, hipStreamCreateWithFlags (&h->aux, hipStreamNonBlocking));
+        hipStream_t side = fork ? h->side : h->stream, aux = fork ? h->aux : h->stream;
+        if (fork) { HIPCHK (h, hipEventRecord (h->ev_fork, h->stream)); HIPCHK (h, hipStreamWaitEvent (aux, h->ev_fork, 0)); }
         if (P.any_rans) {
-            KLAUNCH_ON (h, side, k_hist, dim3 (nl, GZ_HIST_CHUNKS), dim3 (256), GZ_HIST_LDS, d_leaves);
-            KLAUNCH_ON (h, side, k_rans_table, dim3 (nl), dim3 (256), 20480, d_leaves, (const GzLogTable *)h->d_logs);
-            KLAUNCH_ON (h, side, k_rans_encode, dim3 (nl), dim3 (64), GZ_RANS_ENC_LDS, d_leaves);
+            KLAUNCH_ON (h, aux, k_hist, dim3 (nl, GZ_HIST_CHUNKS), dim3 (256), GZ_HIST_LDS, d_leaves);
+            KLAUNCH_ON (h, aux, k_rans_table, dim3 (nl), dim3 (256), 20480, d_leaves, (const GzLogTable *)h->d_logs);
+            KLAUNCH_ON (h, aux, k_rans_encode, dim3 (nl), dim3 (64), GZ_RANS_ENC_LDS, d_leaves);
         }
         if (A.np) {
             const uint32_t grid_y = GZ_MODEL_GRID_Y + (P.rle_list.empty () ? 0 : GZ_MODEL_GRID_RUN);
@@ -757,72 +698,73 @@ static int launch_encode (GzHandle *h, Plan &P, GzdStream *d_streams, GzdLeaf *d
                 if (P.unpacked) KLAUNCH (h, k_arith_model<false>, GZ_XCD_DIM (A.np, grid_y), dim3 (64), GZ_MODEL_LDS, d_leaves, A.d_plain, A.np, 0u, 0xffffffffu, 0u);
                 else            KLAUNCH (h, k_arith_model<true>,  GZ_XCD_DIM (A.np, grid_y), dim3 (64), GZ_MODEL_LDS, d_leaves, A.d_plain, A.np, 0u, 0xffffffffu, 0u);
                 KLAUNCH (h, k_arith_chain, dim3 ((A.np + GZ_CHAIN_WAVES - 1) / GZ_CHAIN_WAVES), dim3 (64 * GZ_CHAIN_WAVES), 64,
-                         d_leaves, A.d_plain, A.np, (const uint32_t *)NULL, (const uint32_t *)NULL, h->d_fail, (uint32_t *)NULL, 0u);
+                         d_leaves, A.d_plain, A.np, 0u, 0xffffffffu, (const uint32_t *)NULL, 0u, h->d_fail);
             }
             else {
-                HIPCHK (h, hipEventRecord (h->ev_model_fork, h->stream));        // (after k_leaf_prep)
-                HIPCHK (h, hipStreamWaitEvent (h->stream4, h->ev_model_fork, 0));
-                HIPCHK (h, hipStreamWaitEvent (h->stream7, h->ev_model_fork, 0));
-                // the sort of a chunk needs nothing from the models: with many leaves it runs ahead on its own stream.
-                // (Tried: the leaves' models as two groups on two streams, each with its own progress counter, so that one group's
-                //  launch fills the tail of the other's - no gain (33.8 vs 33.9 ms; 4 M pairs 84.9 vs 80.6): the model kernels
-                //  are short of issue slots, not of waves.)
+                // The long leaves, per position chunk: sort -> models (this stream) -> chain (`side`, behind the models' event) -> `low` (`aux`, behind the
+                // chain's), so that the chain of chunk k runs beside the models of the chunks behind it and the `low` kernels of the ones in front.
+                // What a stream waits for was always queued before: streams that share a hardware queue get slower, never stuck.
                 if (A.n_chunks > GZ_MAX_CHUNKS) return GZ_ERR;
+                HIPCHK (h, hipEventRecord (h->ev_events, h->stream));            // (the run-length variant's leaves have their lengths)
                 // (wide alphabets: the symbols that follow each context byte anywhere in the leaf, before the first chunk's models)
-                static const uint32_t sort_ahead_min = getenv ("GZ_SORT_AHEAD_MIN") ? (uint32_t)atoi (getenv ("GZ_SORT_AHEAD_MIN")) : 256u;
-                hipStream_t sort_stream = A.nbig > sort_ahead_min ? h->stream7 : h->stream4;   // (measured: 702 leaves 84.0 -> 80.6 ms; 176 leaves 33.9 -> 34.2: the sort then only takes compute units from the models)
-                if (A.no1) KLAUNCH_ON (h, sort_stream, k_ctx_succ, dim3 (A.nbig, (P.max_arith_n + GZ_SUCC_SPAN - 1) / GZ_SUCC_SPAN), dim3 (256), 8192, d_leaves, A.d_big);
-                for (uint32_t k = 0; k < A.n_chunks; k++) {
+                if (A.no1) KLAUNCH (h, k_ctx_succ, dim3 (A.nbig, (P.max_arith_n + GZ_SUCC_SPAN - 1) / GZ_SUCC_SPAN), dim3 (256), 8192, d_leaves, A.d_big);
+                GzHandle::ProfRec chain_rec; chain_rec.name = "k_arith_chain";   // (gz_profile: a batch's chain is one entry, from its first chunk to its last)
+                if (h->profiling) { chain_rec.a = gz_event_get (h); chain_rec.b = gz_event_get (h); }
+                // One chain launch takes several chunks where the models are ahead of it anyhow (they need about half the chain's time per chunk): half
+                // as many as lie behind it, and towards the end half of what is left, so that neither the lead-in nor the `low` kernels of the last
+                // launch get longer. A launch costs ~12 us and, where it asks for whole compute units, up to 0.3 ms until one is free. (Default step, the
+                // chain / the step: a launch per chunk 39.3 / 43.1 ms, a third 36.1 / 39.2, half 35.7 / 38.9, as many 37.0 / 40.1.)
+                uint32_t used = 0, gi = 0;
+                while (used < A.n_chunks && A.bounds[used] < P.max_arith_n) used++;
+                std::vector<uint32_t> groups (1, 0u);                            // launch g: chunks groups[g] .. groups[g + 1] - 1
+                for (uint32_t c = 0; c < used; groups.push_back (c)) c += std::max (std::min (c, used - c) / 2, 1u);
+                const uint32_t chain_wgs = (A.nbig + GZ_CHAIN_WAVES - 1) / GZ_CHAIN_WAVES;
+                // (a whole compute unit each only while that leaves three quarters of them to the rest)
+                const uint32_t chain_lds = chain_wgs <= (uint32_t)h->n_cu / 4 ? GZ_CHAIN_LDS : 64;
+                for (uint32_t k = 0; k < used; k++) {
                     const uint32_t p0 = A.bounds[k], len = A.bounds[k + 1] - p0;
-                    if (p0 >= P.max_arith_n) break;
                     const uint32_t span = P.max_arith_n - p0 < len ? P.max_arith_n - p0 : len;
                     // (the leaves of small alphabets: sort, models and records of the chunk in one kernel, in front of the others' sort)
-                    if (h->tile_models) KLAUNCH_ON (h, h->stream4, k_arith_model_tiled, dim3 (A.nbig), dim3 (64 * GZ_TM_WAVES), GZ_TM_LDS, d_leaves, A.d_big, p0, len, h->tm_dbg);
-                    if ((rc = sort_chunk (sort_stream, A.d_big, A.nbig, p0, len, span, k)) != GZ_OK) return rc;
-                    HIPCHK (h, hipEventRecord (h->ev_sort[k], sort_stream));
-                    HIPCHK (h, hipStreamWaitEvent (h->stream4, h->ev_sort[k], 0));
-                    if (P.unpacked) KLAUNCH_ON (h, h->stream4, k_arith_model<false>, GZ_XCD_DIM (A.nbig, grid_y), dim3 (64), GZ_MODEL_LDS, d_leaves, A.d_big, A.nbig, p0, len, k);
-                    else            KLAUNCH_ON (h, h->stream4, k_arith_model<true>,  GZ_XCD_DIM (A.nbig, grid_y), dim3 (64), GZ_MODEL_LDS, d_leaves, A.d_big, A.nbig, p0, len, k);
-                    if (!h->debug_starve_chain) hipLaunchKernelGGL (k_arith_progress, dim3 (1), dim3 (1), 0, h->stream4, A.d_progress, k + 1);
-                }
-#ifdef GZ_SEQUENTIAL_STREAMS
-                if ((rc = arith_launch_chain (h, A, d_leaves)) != GZ_OK) return rc;
-#endif
-                // (the short leaves are queued BEFORE the gates below: streams share hardware queues, a gate spins until the chain is through
-                //  its chunk, and whatever is queued behind a gate in the same hardware queue waits with it - one VCF VBlock's 7.5 M-symbol
-                //  stripe planes, "short" next to a 30 M-entry b250, started 2.8 s late, after the long chain had finished)
-                if (A.nsmall) {
-                    HIPCHK (h, hipStreamWaitEvent (h->stream5, h->ev_model_fork, 0));
-                    if (h->tile_models) KLAUNCH_ON (h, h->stream5, k_arith_model_tiled, dim3 (A.nsmall), dim3 (64 * GZ_TM_WAVES), GZ_TM_LDS, d_leaves, A.d_small, 0u, 0xffffffffu, h->tm_dbg);
-                    if ((rc = sort_chunk (h->stream5, A.d_small, A.nsmall, 0u, 0xffffffffu, A.chunk, 0u)) != GZ_OK) return rc;
-                    if (P.unpacked) KLAUNCH_ON (h, h->stream5, k_arith_model<false>, GZ_XCD_DIM (A.nsmall, grid_y), dim3 (64), GZ_MODEL_LDS, d_leaves, A.d_small, A.nsmall, 0u, 0xffffffffu, 0u);
-                    else            KLAUNCH_ON (h, h->stream5, k_arith_model<true>,  GZ_XCD_DIM (A.nsmall, grid_y), dim3 (64), GZ_MODEL_LDS, d_leaves, A.d_small, A.nsmall, 0u, 0xffffffffu, 0u);
-                    KLAUNCH_ON (h, h->stream5, k_arith_chain, dim3 ((A.nsmall + GZ_CHAIN_WAVES - 1) / GZ_CHAIN_WAVES), dim3 (64 * GZ_CHAIN_WAVES), GZ_KEEP_OFF_LDS,
-                                d_leaves, A.d_small, A.nsmall, (const uint32_t *)NULL, (const uint32_t *)NULL, h->d_fail, (uint32_t *)NULL, 0u);
-                    if (A.nlb_small) {
-                        KLAUNCH_ON (h, h->stream5, k_chain_expand, dim3 (A.nlb_small), dim3 (64), GZ_EXPAND_LDS, d_leaves, A.d_lb_small, (const uint32_t *)NULL, 0u, h->debug_chain_fault);
-                        KLAUNCH_ON (h, h->stream5, k_low_scan, dim3 (A.nsmall), dim3 (1024), 8192, d_leaves, A.d_small, 0u, 0xffffffffu);
-                        KLAUNCH_ON (h, h->stream5, k_low_scatter, dim3 (A.nlb_small), dim3 (GZ_LOW_WG), GZ_KEEP_OFF_LDS, d_leaves, A.d_lb_small, (const uint32_t *)NULL, 0u);
+                    if (h->tile_models) KLAUNCH (h, k_arith_model_tiled, dim3 (A.nbig), dim3 (64 * GZ_TM_WAVES), GZ_TM_LDS, d_leaves, A.d_big, p0, len, h->tm_dbg);
+                    if ((rc = sort_chunk (h->stream, A.d_big, A.nbig, p0, len, span, k)) != GZ_OK) return rc;
+                    if (P.unpacked) KLAUNCH (h, k_arith_model<false>, GZ_XCD_DIM (A.nbig, grid_y), dim3 (64), GZ_MODEL_LDS, d_leaves, A.d_big, A.nbig, p0, len, k);
+                    else            KLAUNCH (h, k_arith_model<true>,  GZ_XCD_DIM (A.nbig, grid_y), dim3 (64), GZ_MODEL_LDS, d_leaves, A.d_big, A.nbig, p0, len, k);
+                    if (!h->debug_starve_chain) hipLaunchKernelGGL (k_arith_progress, dim3 (1), dim3 (1), 0, h->stream, A.d_progress, k + 1);
+                    HIPCHK (h, hipEventRecord (h->ev_model[k], h->stream));
+                    if (!k && A.nsmall) {                            // the short leaves, in one piece
+                        HIPCHK (h, hipStreamWaitEvent (side, h->ev_events, 0));
+                        if (h->tile_models) KLAUNCH_ON (h, side, k_arith_model_tiled, dim3 (A.nsmall), dim3 (64 * GZ_TM_WAVES), GZ_TM_LDS, d_leaves, A.d_small, 0u, 0xffffffffu, h->tm_dbg);
+                        if ((rc = sort_chunk (side, A.d_small, A.nsmall, 0u, 0xffffffffu, A.chunk, 0u)) != GZ_OK) return rc;
+                        if (P.unpacked) KLAUNCH_ON (h, side, k_arith_model<false>, GZ_XCD_DIM (A.nsmall, grid_y), dim3 (64), GZ_MODEL_LDS, d_leaves, A.d_small, A.nsmall, 0u, 0xffffffffu, 0u);
+                        else            KLAUNCH_ON (h, side, k_arith_model<true>,  GZ_XCD_DIM (A.nsmall, grid_y), dim3 (64), GZ_MODEL_LDS, d_leaves, A.d_small, A.nsmall, 0u, 0xffffffffu, 0u);
+                        KLAUNCH_ON (h, side, k_arith_chain, dim3 ((A.nsmall + GZ_CHAIN_WAVES - 1) / GZ_CHAIN_WAVES), dim3 (64 * GZ_CHAIN_WAVES), GZ_KEEP_OFF_LDS,
+                                    d_leaves, A.d_small, A.nsmall, 0u, 0xffffffffu, (const uint32_t *)NULL, 0u, h->d_fail);
+                        if (A.nlb_small) {
+                            KLAUNCH_ON (h, side, k_chain_expand, dim3 (A.nlb_small), dim3 (64), GZ_EXPAND_LDS, d_leaves, A.d_lb_small, (const uint32_t *)NULL, 0u, h->debug_chain_fault);
+                            KLAUNCH_ON (h, side, k_low_scan, dim3 (A.nsmall), dim3 (1024), 8192, d_leaves, A.d_small, 0u, 0xffffffffu);
+                            KLAUNCH_ON (h, side, k_low_scatter, dim3 (A.nlb_small), dim3 (GZ_LOW_WG), GZ_KEEP_OFF_LDS, d_leaves, A.d_lb_small, (const uint32_t *)NULL, 0u);
+                        }
                     }
-                    HIPCHK (h, hipEventRecord (h->ev_small, h->stream5));
-                    HIPCHK (h, hipStreamWaitEvent (h->stream, h->ev_small, 0));
+                    if (k + 1 != groups[gi + 1]) continue;
+                    HIPCHK (h, hipStreamWaitEvent (side, h->ev_model[k], 0));
+                    if (!gi && h->profiling) (void)hipEventRecord (chain_rec.a, side);
+                    const uint32_t c0 = A.bounds[groups[gi]];
+                    hipLaunchKernelGGL (k_arith_chain, dim3 (chain_wgs), dim3 (64 * GZ_CHAIN_WAVES), chain_lds, side,
+                                        d_leaves, A.d_big, A.nbig, c0, A.bounds[k + 1] - c0, (const uint32_t *)A.d_progress, k + 1, h->d_fail);
+                    HIPCHK (h, hipEventRecord (h->ev_chain[gi], side));
+                    gi++;
                 }
-                // the `low` kernels of the long leaves follow the chain: a one-thread gate holds their stream until every
-                // leaf is through chunk k; count / scan / scatter of that chunk then run beside the chain's next chunk
-                HIPCHK (h, hipStreamWaitEvent (h->stream6, h->ev_model_fork, 0));
-                for (uint32_t k = 0; k < A.n_chunks; k++) {
-                    const uint32_t p0 = A.bounds[k], len = A.bounds[k + 1] - p0;
-                    if (p0 >= P.max_arith_n) break;
-                    const uint32_t span = P.max_arith_n - p0 < len ? P.max_arith_n - p0 : len;
+                if (h->profiling) { (void)hipEventRecord (chain_rec.b, side); h->prof_open.push_back (chain_rec); }
+                for (uint32_t g = 0; g < gi; g++) {
+                    const uint32_t p0 = A.bounds[groups[g]], len = A.bounds[groups[g + 1]] - p0, span = P.max_arith_n - p0 < len ? P.max_arith_n - p0 : len;
                     const uint32_t wgs = (span + GZ_LOW_SLICE * GZ_LOW_SLICES_PER_WG - 1) / (GZ_LOW_SLICE * GZ_LOW_SLICES_PER_WG);
-                    hipLaunchKernelGGL (k_low_gate, dim3 (1), dim3 (1), 0, h->stream6, (const uint32_t *)(A.d_progress + 16 + k), A.nbig, h->d_fail);
-                    KLAUNCH_ON (h, h->stream6, k_chain_expand, dim3 (A.nbig, wgs), dim3 (64), GZ_EXPAND_LDS, d_leaves, (const GzdLowBlock *)NULL, A.d_big, p0, h->debug_chain_fault);
-                    KLAUNCH_ON (h, h->stream6, k_low_scan, dim3 (A.nbig), dim3 (1024), 8192, d_leaves, A.d_big, p0, len);
-                    KLAUNCH_ON (h, h->stream6, k_low_scatter, dim3 (A.nbig, wgs), dim3 (GZ_LOW_WG), GZ_KEEP_OFF_LDS, d_leaves, (const GzdLowBlock *)NULL, A.d_big, p0);
+                    HIPCHK (h, hipStreamWaitEvent (aux, h->ev_chain[g], 0));
+                    KLAUNCH_ON (h, aux, k_chain_expand, dim3 (A.nbig, wgs), dim3 (64), GZ_EXPAND_LDS, d_leaves, (const GzdLowBlock *)NULL, A.d_big, p0, h->debug_chain_fault);
+                    KLAUNCH_ON (h, aux, k_low_scan, dim3 (A.nbig), dim3 (1024), 8192, d_leaves, A.d_big, p0, len);
+                    KLAUNCH_ON (h, aux, k_low_scatter, dim3 (A.nbig, wgs), dim3 (GZ_LOW_WG), GZ_KEEP_OFF_LDS, d_leaves, (const GzdLowBlock *)NULL, A.d_big, p0);
                 }
-                HIPCHK (h, hipEventRecord (h->ev_low, h->stream6));
-                HIPCHK (h, hipStreamWaitEvent (h->stream, h->ev_chain, 0));
-                HIPCHK (h, hipStreamWaitEvent (h->stream, h->ev_low, 0));
+                // (every digit before k_low_resid; `side` ends with the chain that aux has waited for)
+                HIPCHK (h, hipEventRecord (h->ev_join, aux)); HIPCHK (h, hipStreamWaitEvent (h->stream, h->ev_join, 0));
             }
             if (!A.pipelined) {
                 KLAUNCH (h, k_chain_expand, dim3 (A.nlb), dim3 (64), GZ_EXPAND_LDS, d_leaves, A.d_lb, (const uint32_t *)NULL, 0u, h->debug_chain_fault);
@@ -837,7 +779,7 @@ static int launch_encode (GzHandle *h, Plan &P, GzdStream *d_streams, GzdLeaf *d
                 KLAUNCH (h, k_low_carry, dim3 (A.np), dim3 (64), 0, d_leaves, A.d_plain);
             }
         }
-        if (fork) { HIPCHK (h, hipEventRecord (h->ev_join, side)); HIPCHK (h, hipStreamWaitEvent (h->stream, h->ev_join, 0)); }
+        if (fork) { HIPCHK (h, hipEventRecord (h->ev_join, aux)); HIPCHK (h, hipStreamWaitEvent (h->stream, h->ev_join, 0)); }
     }
     if (n_vbs && h->emit_after) {                    // precompressed sections coded on another handle: only the writer waits for them
         if (!h->ev_other) HIPCHK (h, hipEventCreateWithFlags (&h->ev_other, hipEventDisableTiming));
@@ -1053,8 +995,6 @@ static int gz_sync_do (GzHandle *h)
 {
     HIPCHK (h, hipSetDevice (h->device));
     const hipError_t sync_err = hipStreamSynchronize (h->stream);
-    g_chain_wgs.fetch_sub (h->chain_wgs_held); g_chain_cus.fetch_sub (h->chain_cus_held);
-    h->chain_wgs_held = h->chain_cus_held = 0;
     HIPCHK (h, sync_err);
 #ifdef GZ_MODEL_DEBUG
     if (!h->pending.empty ()) {
@@ -1136,8 +1076,7 @@ static int gz_sync_do (GzHandle *h)
     h->host_tmp.clear ();
     arena_reset (h);
     if (device_failed && !h->in_fallback) {
-        // The persistent chain kernel gave up waiting for the model kernels (kernels serialised by a tool, another tenant holding the hardware
-        // queues, a host that initialised HIP before this library could ask for more queues): every stream / VBlock of this sync is suspect.
+        // The chain found a position chunk whose records the model kernels had not announced: every stream / VBlock of this sync is suspect.
         // The reference's contract is "false only for too small, otherwise it works" (src/compressor.c:89-110): the batches run AGAIN, in the
         // unpipelined order of the same kernels - inputs and outputs are the caller's and still there, the tables too (they are pending) -
         // and the caller gets the result of that run, a warning in gz_last_error and a count in gz_chain_fallbacks.
@@ -1151,8 +1090,8 @@ static int gz_sync_do (GzHandle *h)
         if (rc2 >= 0) rc2 = gz_sync_do (h); else (void)gz_sync_do (h);
         h->in_fallback = false;
         h->chain_fallbacks++;
-        if (rc2 >= 0) h->warn = "warning: the arithmetic coder's persistent chain kernel never heard from the model kernels (kernels serialised by a tool? "
-                                "too few hardware queues?); the batch was run again unpipelined (GZ_NO_PIPELINE=1 selects that order from the start)";
+        if (rc2 >= 0) h->warn = "warning: the arithmetic coder's chain did not find the model kernels' records of a position chunk; "
+                                "the batch was run again unpipelined (GZ_NO_PIPELINE=1 selects that order from the start)";
         return rc2;
     }
     if (device_failed) {

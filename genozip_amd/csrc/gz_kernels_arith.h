@@ -17,7 +17,7 @@
 //                  the high word of a double.
 //   k_arith_chain  what is truly serial: range -> range / tot * freq -> renormalise. One wave per leaf, three vector
 //                  instructions per symbol in double precision, the state hopping a lane per symbol (gz_chain_asm.h);
-//                  persistent, following the models position chunk by chunk.
+//                  launched per position chunk, behind the models of it.
 //   k_low_*        low += cum * r is a big-number addition and addition is associative: one thread per symbol adds its
 //                  bytes at the output position given by a prefix sum of the shift counts; then carries.
 #pragma once
@@ -1342,7 +1342,7 @@ __global__ void __launch_bounds__(64 * GZ_TM_WAVES) k_arith_model_tiled (GzdLeaf
 //                  a 9th bit) at its absolute output position (k_chain_expand / k_low_scan: a prefix sum of the k's;
 //                  k_low_scatter), k_low_resid adds what is left in each window where the following slices' bytes
 //                  go, and k_low_norm normalises the digits: carries ripple left inside a tile and, very rarely, across.
-//                  The first three follow the chain chunk by chunk (k_low_gate), the last two run once at the end.
+//                  The first three follow the chain chunk by chunk, the last two run once at the end.
 // This reproduces RC_ShiftLow's cache / pending-0xFF bookkeeping (c_range_coder.h:70-88) exactly: that logic is just
 // a lazy form of the same addition ("[0, T1, T2, ...] plus 1 at the byte before every shift that saw a carry").
 typedef uint32_t gz_u32x4 __attribute__((vector_size (16)));
@@ -1363,33 +1363,17 @@ __device__ static inline uint32_t d_chain_step (uint32_t &rlo, uint32_t &rhi, ui
     return r;
 }
 
-// positions [p0, p0 + chunk) (p0 and chunk are multiples of 256)
-// Four leaves per workgroup, one per wave (= one per SIMD). For the long leaves the kernel is PERSISTENT: it is launched
-// at the start of the step, asks for (nearly) the whole LDS of a compute unit although it uses none - so that no
-// workgroup of another kernel that needs LDS fits beside it and the chain waves, the critical path of the whole step,
-// share instruction fetch and issue with nobody - and then follows the model kernels chunk by chunk: `progress` is the
-// number of position chunks whose records are complete (written by k_arith_progress, which the host queues behind every
-// model launch). Records are only ever read after their chunk was announced, and never before by this kernel (the
-// block requested ahead stays inside the announced chunks), so no stale copy of them can sit in a cache on the way.
+// Four leaves per workgroup, one per wave (= one per SIMD). The long leaves take one launch per position chunk, behind an event the host
+// records after that chunk's models and in front of the one its `low` kernels wait for. The state travels from launch to launch in the
+// checkpoint both ends of a chunk share. No kernel waits on the device for another one: streams may share a hardware queue, and a wave that
+// waits for work queued behind it would wait for ever.
 #ifndef GZ_CHAIN_WAVES                   // (-DGZ_CHAIN_WAVES=1 / 2: a leaf or two per workgroup - measured, round 5: 42.7 - 42.9 ms per default step with 1, 2 or 4)
 #define GZ_CHAIN_WAVES 4
 #endif
-#define GZ_CHAIN_LDS   (156 * 1024)
 
+// behind the models of every position chunk: `chunks_done` chunks' records are complete. The chain's launch of a chunk looks at it once - a
+// chunk that was not announced (models that never ran) fails the batch instead of coding from records that are not there
 __global__ void k_arith_progress (uint32_t *progress, uint32_t chunks_done) { *progress = chunks_done; }
-
-// (bounded: if the models never report - a failed launch - the chain gives up after a few seconds instead of hanging
-//  the device; the leaf is then flagged and its stream fails)
-__device__ static inline bool d_wait_progress (const uint32_t *progress, uint32_t want)
-{
-    for (uint32_t spins = 0; __atomic_load_n (progress, __ATOMIC_RELAXED) < want; spins++) {
-        if (spins > 8000000u) return false;
-        __builtin_amdgcn_s_sleep (16);
-    }
-    __atomic_thread_fence (__ATOMIC_ACQUIRE);
-    gz_scalar_cache_inv ();
-    return true;
-}
 
 // positions [i0, i1) one symbol at a time in the plain formulation (the end of a leaf that does not fill a block of the loop; i0 a
 // multiple of 64): 64 records per trip to memory, fetched by the lanes and handed out by readlane; the state before every 64th
@@ -1418,58 +1402,25 @@ __device__ static __forceinline__ void d_chain_chunk (uint32_t &rlo, uint32_t &r
     if (!lane) gz_stg_u32x2 (ck + 2 * ((p1 + 63) >> 6), rlo, rhi);
 }
 
-// progress == NULL: everything is there already, one piece (bounds is ignored). bounds [0 .. n_chunks]: where the position chunks start (the
-// first ones are shorter than the rest: the first chunk's sort + models are the lead-in of the long streams - gz_host.cpp, arith_pipe_setup)
-__device__ static __forceinline__ void d_arith_chain (GzdLeaf *leaves, const uint32_t *list, uint32_t n_list, const uint32_t *progress, const uint32_t *bounds,
-                                                      uint32_t *fail, uint32_t *done, uint32_t n_chunks)
+// positions [p0, p0 + len) of every listed leaf (p0: a multiple of 64). progress: NULL, or where `want` chunks must have been announced
+__global__ void __launch_bounds__(64 * GZ_CHAIN_WAVES) k_arith_chain (GzdLeaf *leaves, const uint32_t *list, uint32_t n_list, uint32_t p0, uint32_t len,
+                                                                      const uint32_t *progress, uint32_t want, uint32_t *fail)
 {
     const uint32_t li = blockIdx.x * GZ_CHAIN_WAVES + (threadIdx.x >> 6);
     if (li >= n_list) return;
     __builtin_amdgcn_s_setprio (3);
     gz_f64_round_toward_zero ();
     const int lane = threadIdx.x & 63;
-    if (progress && !d_wait_progress (progress, 1)) { if (!lane) *fail = 1; return; }   // (the leaf table itself is only final once the models have started)
     GzdLeaf &L = leaves[list[li]];
-    if (!L.active || L.engine != GZ_ENG_ARITH || !L.arith_n) {
-        if (done && !lane) for (uint32_t k = 0; k < n_chunks; k++) atomicAdd (&done[k], 1u);   // (the low kernels count leaves per chunk)
-        return;
-    }
+    if (progress && *progress < want) { if (!lane) { L.overflow = 2; *fail = 1; } return; }
+    if (!L.active || L.engine != GZ_ENG_ARITH) return;
     const uint32_t n = d_uniform (L.arith_n);
+    if (p0 >= n) return;
     const uint8_t *triples = d_uniform_ptr (L.triples);        // (wave-uniform: keep them in scalar registers)
     uint32_t *ck = d_uniform_ptr ((uint32_t *)L.ckpt);          // (checkpoints: the state before every 64th symbol, 8 bytes each)
     uint32_t rlo = GZ_CHAIN_R0_LO, rhi = GZ_CHAIN_R0_HI;
-    if (!progress) d_chain_chunk (rlo, rhi, lane, 0, n, triples, ck);
-    else
-        for (uint32_t k = 0; k < n_chunks; k++) {
-            const uint32_t p0 = d_uniform (bounds[k]), pe = d_uniform (bounds[k + 1]);
-            if (p0 >= n) break;
-            if (k && !d_wait_progress (progress, k + 1)) { if (!lane) { L.overflow = 2; *fail = 1; } break; }
-            d_chain_chunk (rlo, rhi, lane, p0, pe < n ? pe : n, triples, ck);
-            if (done) {                                        // this leaf's checkpoints of chunk k are final: tell the low kernels
-                __threadfence ();                              // (the loop has waited for its own stores, the fence waits for the compiler's)
-                if (!lane) {
-                    atomicAdd (&done[k], 1u);
-                    if (n <= pe) for (uint32_t k2 = k + 1; k2 < n_chunks; k2++) atomicAdd (&done[k2], 1u);   // (a short leaf has no later chunks)
-                }
-            }
-        }
-}
-
-__global__ void __launch_bounds__(64 * GZ_CHAIN_WAVES) k_arith_chain (GzdLeaf *leaves, const uint32_t *list, uint32_t n_list, const uint32_t *progress,
-                                                                      const uint32_t *bounds, uint32_t *fail, uint32_t *done, uint32_t n_chunks)
-{
-    d_arith_chain (leaves, list, n_list, progress, bounds, fail, done, n_chunks);
-}
-
-// One thread: holds its stream until all `want` leaves of the persistent chain have finished a position chunk (the low
-// kernels of that chunk are queued behind it). Bounded like d_wait_progress.
-__global__ void k_low_gate (const uint32_t *done, uint32_t want, uint32_t *fail)
-{
-    for (uint32_t spins = 0; __atomic_load_n (done, __ATOMIC_RELAXED) < want; spins++) {
-        if (spins > 8000000u) { *fail = 1; return; }
-        __builtin_amdgcn_s_sleep (32);
-    }
-    __atomic_thread_fence (__ATOMIC_ACQUIRE);
+    if (p0) { rlo = d_uniform (ck[2 * (p0 >> 6)]); rhi = d_uniform (ck[2 * (p0 >> 6) + 1]); }
+    d_chain_chunk (rlo, rhi, lane, p0, n - p0 < len ? n : p0 + len, triples, ck);
 }
 
 // ---- low: a big-number sum, one thread per symbol -----------------------------------------------------------------

@@ -957,8 +957,8 @@ extern "C" int gz_fastq_zip_seg (GzZipFile *f, uint8_t *text, uint64_t text_len,
     // (not decided yet whether QUAL goes through DOMQ: both forms are tried, the read-back says which one counts)
     if (want_trial && qmode0) ZCHK (add_trials (K.domq[0].out[0], (const uint32_t *)&d_domqres[0].qual_len, 1));
     // The columns' kernels (line 1 -> items -> contexts) fill the device for ~2.5 ms of a 1 M-pair file. Queued HERE - behind the gathers, in front of
-    // the launch of the long streams - they are what the persistent chain's workgroups (a whole compute unit each) wait for before they can start at
-    // all: measured, the chain kernel started executing ~3.3 ms into the default step although it was launched at ~1.6. With few VBlocks, whose step is
+    // the launch of the long streams - they are what those streams' first models and the chain's workgroups (a whole compute unit each) wait for before
+    // they can start at all: ~1.7 ms later in the default step. With few VBlocks, whose step is
     // the latency of the long chains, they are therefore queued AFTER the long streams' launch (defer_columns): the main path that needs them has 20 ms
     // of slack there. With many VBlocks (the streamed form) the device's time is what counts and they go first, as they always did.
     const size_t NCJ = col_jobs.size ();

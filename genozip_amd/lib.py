@@ -7,11 +7,10 @@ is only ever loaded by tests, through the explicit `path` argument.)
 import ctypes as C
 import os
 
-# The library runs its kernels on ~14 HIP streams per pair of handles, some of which hold one-thread gate kernels that wait for the range
-# coder's long chains. The HIP runtime maps all streams onto 4 hardware queues by default, and whatever shares a queue with a gate waits
-# with it. 8 queues: measured 4 / 6 / 8 / 12 / 16 / 24 - with one call in flight 8 and 12 are the same (default step 46.2 vs 46.5 ms, streamed
-# 167 vs 167 ms per two calls), with two calls in flight 12 is much slower (214 vs 177 ms: beyond 8 the runtime time-slices the queues,
-# whole queues stand still for ~11 ms at a time) - DESIGN.md section 0. The variable is read when the HIP runtime starts: it has to be in the
+# The library runs its kernels on six HIP streams per pair of handles, ordered by events. The HIP runtime maps all streams of a process onto 4
+# hardware queues by default, and what shares a queue runs in the order it was queued. 8 queues give each stream its own: default step 39.2 ms with 8
+# and 39.1 with 4, binned FASTQ 24.3 / 27.7, BAM 26.9 / 33.5, streamed 140 - 147 / 141 - 148. (More than 8: the runtime time-slices them once two calls
+# are in flight, whole queues stand still for ~11 ms at a time.) The variable is read when the HIP runtime starts: it has to be in the
 # environment before the first HIP call of the process (the library's own constructor sets it too, for C hosts); a value the host set wins.
 os.environ.setdefault("GPU_MAX_HW_QUEUES", "8")
 

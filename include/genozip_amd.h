@@ -53,8 +53,9 @@ typedef struct GzHandle GzHandle;   /* stands in for VBlockP: owns the HIP strea
 /* device = HIP device ordinal; hip_stream = a hipStream_t to run on, or NULL for a private stream.
  * Fails (returns NULL, *err set) when no gfx950-capable device / runtime is present: there is NO CPU fallback. */
 GzHandle *gz_create (int device, void *hip_stream, int *err);
-/* the same with all streams (but the range coder chain's) at the lowest priority: for long-running batches that run beside another
- * handle's short ones (the VBlock compute driver codes the long QUAL streams on such a handle) */
+/* the same for long-running batches that run beside another handle's short ones (the VBlock compute driver codes the long QUAL streams on
+ * such a handle). All streams of every handle have the default priority, and no kernel waits on the device for another one: the order
+ * between streams is that of events, whatever hardware queues they share. */
 GzHandle *gz_create_background (int device, int *err);
 void      gz_destroy (GzHandle *h);
 int       gz_sync (GzHandle *h);
@@ -64,15 +65,16 @@ const char *gz_version (void);
  * the handle's stream; gz_sync() folds them into per-kernel totals (this is the reference's --show-time /
  * START_TIMER..COPY_TIMER instrumentation, src/profiler.h:96-166, re-expressed for a GPU stream).
  * gz_profile_get(idx) enumerates the accumulated entries until it returns 0. enable = 2: only the launches of the two kernels a step can
- * be as long as (k_arith_chain, k_arith_model) - the events of ALL launches cost the host as much as the launches do (~700 a step). */
+ * be as long as (k_arith_chain, k_arith_model) - the events of ALL launches cost the host as much as the launches do (~700 a step).
+ * The chain of a batch's long leaves goes out in several launches, one behind the other: they count as one, from the first to the last. */
 void gz_profile (GzHandle *h, int enable, int reset);
 int  gz_profile_get (GzHandle *h, int idx, char *name, int name_cap, double *total_ms, int *launches);
 /* the longest single launch of entry idx of the walk begun with gz_profile_get (h, 0, ...) */
 int  gz_profile_get_max (GzHandle *h, int idx, double *max_ms);
 /* the HIP stream work is queued on (a hipStream_t) - for timing with HIP events on the right stream */
 void     *gz_stream (GzHandle *h);
-/* How often gz_sync ran a batch a second time, unpipelined, because the arithmetic coder's persistent chain kernel never heard from the
- * model kernels it follows (kernels serialised by a profiling tool, too few hardware queues, another tenant). The results are those of the
+/* How often gz_sync ran a batch a second time, unpipelined, because the arithmetic coder's chain found a position chunk whose records the
+ * model kernels had not announced (a check behind every chunk's models; nothing but a failed launch should make it fail). The results are those of the
  * second run - the reference's COMPRESS contract: false only for "too small" (src/compressor.c:89-110). The return code is that of the second
  * run and gz_last_error is left alone; gz_last_warning says what happened (a string that stays until the next fallback).
  * CONTRACT for the asynchronous batch calls (gz_codec_compress_batch, gz_vb_compress_batch): the second run reads the caller's tables and INPUT

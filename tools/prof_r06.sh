@@ -1,5 +1,5 @@
 # round 6: rocprofv3 kernel stats + HBM counters of the default bench command (one gpurun call). PMC passes: separate runs, serialised
-# kernels (GZ_NO_PIPELINE: no persistent kernel), codecs pinned (no trial compressions), as tools/history/prof_round2.sh
+# kernels (GZ_NO_PIPELINE), codecs pinned (no trial compressions), as tools/history/prof_round2.sh
 set -x
 OUT=/root/repo/gpurun_out/prof_r06; mkdir -p $OUT; cd /tmp; export TMPDIR=/tmp
 timeout 900 rocprofv3 --kernel-trace --stats --output-format csv -d $OUT/trace -o r06 -- python /root/repo/bench.py --steps 3 --warmup 1 --no-cpu --warm-steps 0 > $OUT/bench_stats.json 2> $OUT/trace.err

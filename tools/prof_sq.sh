@@ -1,5 +1,5 @@
 # SQ counters of the hot kernels (where do a kernel's wave cycles go: issuing, waiting for an instruction's operands, parked at s_waitcnt):
-# separate --pmc passes with the kernels serialised (GZ_NO_PIPELINE: no persistent chain), per configuration.   usage: prof_sq.sh <tag> <bench args ...>
+# separate --pmc passes with the kernels serialised (GZ_NO_PIPELINE), per configuration.   usage: prof_sq.sh <tag> <bench args ...>
 set -x
 TAG=$1; shift
 OUT=/root/repo/gpurun_out/sq_$TAG; mkdir -p $OUT; cd /tmp; export TMPDIR=/tmp

@@ -54,7 +54,7 @@ for r in rows:
                                       "dispatches_per_step": r["dispatches"] / STEPS, "traffic_bytes": int(per_dispatch),
                                       "traffic_bytes_per_step": int(per_dispatch * r["dispatches"] / STEPS)}
 json.dump({"workload": workload, "source": "GZ_NO_PIPELINE=1 GZ_ZIP_NO_OVERLAP=1 rocprofv3 --pmc FETCH_SIZE / --pmc WRITE_SIZE (separate passes) of: python bench.py --steps 2 --warmup 1 --no-cpu "
-                     "--pin-codecs. (Counter collection serialises kernels, which the persistent chain kernel cannot live with: GZ_NO_PIPELINE runs the "
+                     "--pin-codecs. (Counter collection serialises kernels anyway: GZ_NO_PIPELINE runs the "
                      "same kernels over the same data one after the other - per step the bytes are the same, only the number of launches they are "
                      "spread over differs, hence traffic_bytes_per_step.)",
            "correction": "traffic = 2 x FETCH_SIZE x 1024 + WRITE_SIZE x 1024 (gfx950 FETCH_SIZE half-count; WRITE_SIZE uncalibrated)", "kernels": pmc},

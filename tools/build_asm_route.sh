@@ -7,7 +7,7 @@ ROOT=$(cd "$(dirname "$0")/.." && pwd)
 OUT=$1; MODE=${2:-align}; shift; [ $# -gt 0 ] && shift
 T=$(mktemp -d); trap 'rm -rf $T' EXIT
 LLVM=/opt/rocm/lib/llvm/bin
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-value -I $ROOT/genozip_amd/csrc $*"
+FLAGS="--offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC -ffp-contract=off -Wno-unused-value -I $ROOT/genozip_amd/csrc $*"
 /opt/rocm/bin/hipcc $FLAGS -x hip $ROOT/genozip_amd/csrc/gz_host.cpp --cuda-device-only -S -o $T/dev.s
 if [ "$MODE" = align ]; then python3 $ROOT/tools/align_asm.py $T/dev.s $T/dev_al.s > $T/align.log; tail -1 $T/align.log; else cp $T/dev.s $T/dev_al.s; fi
 $LLVM/clang -x assembler -target amdgcn-amd-amdhsa -mcpu=gfx950 -c $T/dev_al.s -o $T/dev.o

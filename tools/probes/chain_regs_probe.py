@@ -3,7 +3,7 @@
 operand registers, 13.8 with the product's rotating ones, 15.1 with hops, loads and checkpoints)? Writes one .hip file with a kernel per
 variant of the loop body - timing only, the values are whatever they are - and a main() that prints clocks per symbol for each.
 
-    python tools/probes/chain_regs_probe.py /tmp/chain_regs_probe.hip && hipcc --offload-arch=gfx950 -O2 /tmp/chain_regs_probe.hip -o tools/probes/chain_regs_probe.bin
+    python tools/probes/chain_regs_probe.py /tmp/chain_regs_probe.hip && hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 /tmp/chain_regs_probe.hip -o tools/probes/chain_regs_probe.bin
     (GPU box)  tools/probes/chain_regs_probe.bin
 """
 import sys

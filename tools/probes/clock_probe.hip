@@ -1,5 +1,5 @@
 // what clock does a nearly idle MI355X give ONE wave? s_memtime (shader clock) against s_memrealtime (100 MHz) around a chain of dependent
-// integer adds, alone and beside a grid that keeps every compute unit busy:   hipcc --offload-arch=gfx950 -O2 clock_probe.hip -o clock_probe
+// integer adds, alone and beside a grid that keeps every compute unit busy:   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 clock_probe.hip -o clock_probe
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>

@@ -3,7 +3,7 @@
 of one kind or a short pattern, one wave on an idle device (timing only). Behind tools/probes/chain_regs_probe.py's finding that an 8-byte
 instruction at an odd word costs a clock more, and tools/align_asm.py's A / B that found the decoder 5 % SLOWER with its 4-byte VALU
 instructions promoted to 8-byte ones.
-    python tools/probes/issue_probe.py /tmp/issue_probe.hip && hipcc --offload-arch=gfx950 -O2 /tmp/issue_probe.hip -o tools/probes/issue_probe.bin
+    python tools/probes/issue_probe.py /tmp/issue_probe.hip && hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 /tmp/issue_probe.hip -o tools/probes/issue_probe.bin
 """
 import sys
 

@@ -1,5 +1,5 @@
 // dependent-chain cost of the instruction sequences a one-wave serial decoder is made of (gfx950, one wave on an idle chip), in shader clocks per
-// link of the chain:   hipcc --offload-arch=gfx950 -O2 lat_probe.hip -o lat_probe && ./lat_probe
+// link of the chain:   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 lat_probe.hip -o lat_probe && ./lat_probe
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>

@@ -8,7 +8,7 @@
 //   * k_chain_f64    a compiler-scheduled four-instruction form with scalar-register operands (how it started: exact, but its
 //                    scalar loads cannot be waited for one at a time)
 //   * k_chain_int    rounds 1-3's integer form, scalar operands, without the L2 touch of the product's old loop
-// build: hipcc -O3 --offload-arch=gfx950 -ffp-contract=off -I tools tools/ubench_chain_f64.hip -o tools/ubench_f64.bin
+// build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off -I tools tools/ubench_chain_f64.hip -o tools/ubench_f64.bin
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>

@@ -1,5 +1,5 @@
 // issue-interval probes for one wave on gfx950: dependent chains of single instructions and of the range coder step
-// build: hipcc -O3 --offload-arch=gfx950 tools/ubench_issue.hip -o tools/ubench_issue.bin
+// build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/ubench_issue.hip -o tools/ubench_issue.bin
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>

@@ -2,7 +2,7 @@
 // (the guide: "WRITE_SIZE is uncalibrated: calibrate on a known byte count in your own access pattern").
 // The access patterns are the model kernel's: wave (c, b) - context c of S, batch b - stores the records of positions (64 b + lane) S + c,
 // i.e. S waves fill S neighbouring records each; grid order decides whether those S waves sit on one XCD (one L2) or on S of them.
-// build: hipcc -O3 --offload-arch=gfx950 tools/ubench_scatter.hip -o tools/ubench_scatter.bin     run: tools/ubench_scatter.bin [MiB]
+// build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/ubench_scatter.hip -o tools/ubench_scatter.bin     run: tools/ubench_scatter.bin [MiB]
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>

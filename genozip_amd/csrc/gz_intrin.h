@@ -34,18 +34,6 @@ __device__ static inline uint32_t gz_wave_or_scan (uint32_t v)
     return v;
 }
 
-// Pull the 64-byte line at p towards this wave's L2 without ever waiting for it: a plain global load whose result lands in
-// `pit`, a register the caller keeps alive (and untouched) until gz_touch_done. Written as inline asm because the
-// compiler would otherwise either wait for the value where it is consumed or move the load to where it is.
-__device__ static inline void gz_touch (const void *p, uint32_t &pit)
-{
-    asm volatile ("global_load_dword %0, %1, off" : "+v"(pit) : "v"(p) : "memory");
-}
-__device__ static inline void gz_touch_done (uint32_t &pit)
-{
-    asm volatile ("s_waitcnt vmcnt(0)" : "+v"(pit) : : "memory");
-}
-
 // all lanes of the wave have performed their LDS accesses so far before any lane performs a later one (one wave's LDS
 // operations execute in order; this only has to keep the compiler from reordering them)
 __device__ static inline void gz_wave_sync (void) { __builtin_amdgcn_fence (__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier (); }

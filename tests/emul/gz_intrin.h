@@ -5,8 +5,6 @@
 static inline uint32_t gz_mbcnt (uint64_t m) { return (uint32_t)__builtin_popcountll (m & ((1ull << (emu.cur % 64)) - 1)); }
 static inline void gz_wait_scalar_loads (void) {}
 static inline void gz_sched_fence (void) {}
-static inline void gz_touch (const void *p, uint32_t &pit) { pit += *(const volatile uint8_t *)p; }
-static inline void gz_touch_done (uint32_t &) {}
 static inline uint32_t gz_wave_or_scan (uint32_t v)
 {
     const int lane = (int)(emu.cur % 64);

@@ -297,3 +297,20 @@ def test_nothing_writes_through_the_scalar_data_cache():
                     text = open(os.path.join(d, f), errors="replace").read()
                     assert not bad.search(text), os.path.join(d, f)
     assert seen > 50
+
+
+def test_inline_asm_holds_no_load_that_outlives_it():
+    """the compiler takes an asm block's output registers as written at once and as free when unused: a load still in flight at the end of the block
+    would write over whatever lives there by then. Every block with a load in it waits for it in the same block"""
+    csrc = os.path.join(ROOT, "genozip_amd", "csrc")
+    blocks = 0
+    for f in sorted(os.listdir(csrc)):
+        text = open(os.path.join(csrc, f)).read()
+        for m in re.finditer(r"\basm\s*(?:volatile\s*)?\(", text):
+            body = text[m.end():text.index(";", m.end())]
+            if "GZ_CHAIN_F64_ASM" in body:
+                continue                                     # (the loop: the interpreter above sees its loads home)
+            blocks += 1
+            if re.search(r"_load_|_read_|s_memtime|s_load", body):
+                assert "s_waitcnt" in body.split("load")[-1], (f, body)
+    assert blocks >= 3

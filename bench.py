@@ -32,14 +32,16 @@ import subprocess
 import sys
 import time
 
-os.environ.setdefault("GPU_MAX_HW_QUEUES", "8")    # (genozip_amd/lib.py: must be set before the process's first HIP call)
+# the library's recommendation (genozip_amd/lib.py), also where the environment carries the runtime's default of 4: this process is the host, and
+# the choice is the host's. Must be set before the process's first HIP call. (GZ_BENCH_HW_QUEUES: another number, to measure with)
+os.environ["GPU_MAX_HW_QUEUES"] = os.environ.get("GZ_BENCH_HW_QUEUES", "8")
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
 sys.path.insert(0, ROOT)
 
 CHAIN_FLOOR_NS = 5.03           # three dependent vector instructions per symbol at the one-instruction-per-4-clocks issue rate of a wave: 12.07 clocks at 2.4 GHz - what no
                                 # arrangement of this formulation can beat (tools/probes/chain_regs_probe.py: `p_pad0`, profiles/r06_chain_regs_probe_aligned.txt)
-CHAIN_ALONE_NS = 5.41           # k_arith_chain's loop as it is, alone on the device: 13.00 clocks per symbol (profiles/r06_ubench_chain_single.txt; round 5: 6.3, round 4: 6.6)
+CHAIN_ALONE_NS = 5.45           # k_arith_chain's loop as it is, alone on the device: 13.02 clocks per symbol (profiles/ubench_chain_vector_ckpt.txt; round 5: 6.3, round 4: 6.6)
 HBM_PEAK_GBS = 8000.0      # MI355X_MICROARCH.md: HBM3E 8 TB/s spec
 METRIC = "input MB/s compressed (bit-exact .genozip) at 1/2/4/8 GPUs vs CPU ref"
 
@@ -1101,7 +1103,7 @@ def main():
     # QUAL streams + the short-leaf launches of trials and section writer): they overlap, their sum is NOT time on the step's
     # critical path - the LONGEST is (a batch's chunk launches count as one: gz_profile). That one codes the long streams (sections of >= 1 MB); what bounds it is the issue rate
     # of one wave per stream, not HBM: three dependent vector instructions per symbol (12.07 clocks = 5.03 ns at 2.4 GHz: the floor) + a
-    # lane hop every 16 symbols, the checkpoints and the operand loads in the hops' wait states = 13.00 clocks = 5.41 ns with the loop alone
+    # lane hop every 16 symbols, the checkpoints and the operand loads in the hops' wait states = 13.02 clocks = 5.45 ns with the loop alone
     # on the device (tools/ubench_chain_f64.hip; round 5: 15.1, round 4: 15.8, rounds 1-3: seven scalar integer instructions, 12.7 ns).
     # ns_per_symbol below is the time from its first launch to the end of its last / the symbols of its longest stream.
     secs_all = [s for z in z_all for s in walk_sections(z)]

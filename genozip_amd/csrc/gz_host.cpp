@@ -50,6 +50,9 @@ struct ArenaBlock { uint8_t *base; size_t size, used; };
 // loaded before the process's first HIP call; never overrides what the host has set.
 __attribute__((constructor)) static void gz_runtime_env (void) { setenv ("GPU_MAX_HW_QUEUES", "8", 0); }
 
+// compute units that the chains of this process's queued batches ask for as a whole (several handles - one per host thread - share the device)
+static std::atomic<int> g_chain_cus (0);
+
 #define GZ_MAX_CHUNKS 129    // position chunks of the arithmetic coder's pipeline: at most 16 - or GZ_ARITH_CHUNKS - (arith_pipe_setup) + a partial one
 struct GzHandle {
     int device;
@@ -63,6 +66,7 @@ struct GzHandle {
     hipEvent_t ev_fork, ev_join, ev_events;
     hipEvent_t ev_model[GZ_MAX_CHUNKS], ev_chain[GZ_MAX_CHUNKS];   // position chunk k: its records are there / its checkpoints are
     int n_cu = 0;             // compute units of the device
+    int chain_cus_held = 0;   // this handle's share of g_chain_cus, returned at gz_sync
     uint32_t *d_fail = NULL;  // set by a kernel that gave up (the chain of a position chunk whose records were not announced)
     GzHandle *emit_after = NULL;   // the next VBlock batch's section writer waits for this handle's queued work (gz_emit_after)
     GzHandle *emit_after_used = NULL;   // what the batch being queued right now has consumed of it
@@ -224,6 +228,7 @@ static void prof_collect (GzHandle *h);
 extern "C" void gz_destroy (GzHandle *h)
 {
     if (!h) return;
+    g_chain_cus.fetch_sub (h->chain_cus_held); h->chain_cus_held = 0;
     (void)hipSetDevice (h->device);
     (void)hipStreamSynchronize (h->stream);
     prof_collect (h);
@@ -719,8 +724,10 @@ static int launch_encode (GzHandle *h, Plan &P, GzdStream *d_streams, GzdLeaf *d
                 std::vector<uint32_t> groups (1, 0u);                            // launch g: chunks groups[g] .. groups[g + 1] - 1
                 for (uint32_t c = 0; c < used; groups.push_back (c)) c += std::max (std::min (c, used - c) / 2, 1u);
                 const uint32_t chain_wgs = (A.nbig + GZ_CHAIN_WAVES - 1) / GZ_CHAIN_WAVES;
-                // (a whole compute unit each only while that leaves three quarters of them to the rest)
-                const uint32_t chain_lds = chain_wgs <= (uint32_t)h->n_cu / 4 ? GZ_CHAIN_LDS : 64;
+                // (a whole compute unit each only while that leaves three quarters of them to the rest, the chains of the process's other handles counted)
+                uint32_t chain_lds = GZ_CHAIN_LDS;
+                if (g_chain_cus.fetch_add ((int)chain_wgs) + (int)chain_wgs <= h->n_cu / 4) h->chain_cus_held += (int)chain_wgs;
+                else { g_chain_cus.fetch_sub ((int)chain_wgs); chain_lds = 64; }
                 for (uint32_t k = 0; k < used; k++) {
                     const uint32_t p0 = A.bounds[k], len = A.bounds[k + 1] - p0;
                     const uint32_t span = P.max_arith_n - p0 < len ? P.max_arith_n - p0 : len;
@@ -995,6 +1002,7 @@ static int gz_sync_do (GzHandle *h)
 {
     HIPCHK (h, hipSetDevice (h->device));
     const hipError_t sync_err = hipStreamSynchronize (h->stream);
+    g_chain_cus.fetch_sub (h->chain_cus_held); h->chain_cus_held = 0;
     HIPCHK (h, sync_err);
 #ifdef GZ_MODEL_DEBUG
     if (!h->pending.empty ()) {

@@ -80,3 +80,35 @@ def test_one_hardware_queue():
     code = ONE_QUEUE % (ROOT, os.path.join(ROOT, "oracle"), os.path.join(ROOT, "tests"))
     p = subprocess.run([sys.executable, "-u", "-c", code], env=dict(os.environ, GPU_MAX_HW_QUEUES="1"), stdout=subprocess.PIPE, stderr=subprocess.PIPE, timeout=100)
     assert p.returncode == 0 and b"ONE QUEUE OK" in p.stdout, p.stdout.decode()[-1000:] + p.stderr.decode()[-3000:]
+
+
+@pytest.mark.gpu
+def test_handles_of_several_threads(oracle):
+    """six host threads, a handle each, long and short leaves at the same time: more streams than hardware queues, and chains that would ask for
+    more whole compute units than the process gives away - the oracle's bytes on every handle, round after round"""
+    import threading
+    from genozip_amd import synth
+    from genozip_amd.codec import Engine
+    data = [synth.quality_diverse(40 + t, 1500 + 300 * t).tobytes() for t in range(6)]     # 225 - 450 KB: 4 - 7 position chunks
+    want = [[oracle.codec_compress(c, d) for c in (16, 17)] for d in data]
+    bad = []
+
+    def work(t):
+        E = Engine(device=0)
+        try:
+            for rep in range(3):
+                got = E.compress_many([(16, data[t])] * 9 + [(17, data[t])] * 9)
+                if got != [want[t][0]] * 9 + [want[t][1]] * 9:
+                    bad.append((t, rep))
+            if E.L.gz_chain_fallbacks(E.h):
+                bad.append((t, "a batch ran twice"))
+        except Exception as e:                                            # (a thread's exception would go unseen)
+            bad.append((t, repr(e)))
+        finally:
+            E.close()
+    ts = [threading.Thread(target=work, args=(t,)) for t in range(6)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad, bad

@@ -718,7 +718,7 @@ static int launch_encode (GzHandle *h, Plan &P, GzdStream *d_streams, GzdLeaf *d
                 // One chain launch takes several chunks where the models are ahead of it anyhow (they need about half the chain's time per chunk): half
                 // as many as lie behind it, and towards the end half of what is left, so that neither the lead-in nor the `low` kernels of the last
                 // launch get longer. A launch costs ~12 us and, where it asks for whole compute units, up to 0.3 ms until one is free. (Default step, the
-                // chain / the step: a launch per chunk 39.3 / 43.1 ms, a third 36.1 / 39.2, half 35.7 / 38.9, as many 37.0 / 40.1.)
+                // chain / the step: a launch per chunk 39.3 / 43.1 ms, a third 36.0 / 39.2, half 35.7 / 38.9, as many 37.0 / 40.1.)
                 uint32_t used = 0, gi = 0;
                 while (used < A.n_chunks && A.bounds[used] < P.max_arith_n) used++;
                 std::vector<uint32_t> groups (1, 0u);                            // launch g: chunks groups[g] .. groups[g + 1] - 1

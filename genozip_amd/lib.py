@@ -9,7 +9,7 @@ import os
 
 # The library runs its kernels on six HIP streams per pair of handles, ordered by events. The HIP runtime maps all streams of a process onto 4
 # hardware queues by default, and what shares a queue runs in the order it was queued. 8 queues give each stream its own: default step 39.2 ms with 8
-# and 39.1 with 4, binned FASTQ 24.3 / 27.7, BAM 26.9 / 33.5, streamed 140 - 147 / 141 - 148. (More than 8: the runtime time-slices them once two calls
+# and 38.7 with 4, binned FASTQ 24.5 / 27.4, BAM 26.7 / 33.4, VCF 882 / 887, streamed 147 / 141. (More than 8: the runtime time-slices them once two calls
 # are in flight, whole queues stand still for ~11 ms at a time.) The variable is read when the HIP runtime starts: it has to be in the
 # environment before the first HIP call of the process (the library's own constructor sets it too, for C hosts); a value the host set wins.
 os.environ.setdefault("GPU_MAX_HW_QUEUES", "8")
